@@ -46,6 +46,7 @@ typedef struct slm_buf slm_buf;
 typedef struct slm_model slm_model;
 typedef struct slm_session slm_session;
 typedef struct slm_batch slm_batch;
+typedef struct slm_table slm_table;
 
 /* Message of the last failed call on this thread ("" if none). */
 const char* slm_last_error(void);
@@ -161,6 +162,91 @@ int slm_op_attend(slm_ctx* ctx, slm_buf* y, slm_buf* scores, const slm_buf* q, s
  * GPU race. */
 int slm_op_attend_noalloc(slm_ctx* ctx, float* y, const float* q, const float* k, const float* v,
                           const slm_attn* a);
+
+/* ---------------------------------------------------------------------- */
+/* Paged key-value caches.  No counterpart in the reference, whose caches are
+ * one contiguous [key_heads][cap][dh] array per sequence (src/ops.rs:207-227):
+ * here many sequences share one pool of fixed-size pages, one call serves all
+ * of them, pages may hold bf16, and a cache can be brought down to a budget.
+ *
+ * A pool is a pair of buffers, K and V, of pages · key_heads · page · dh
+ * values, laid out [pages][key_heads][page][dh]: f32 values, or bf16 values
+ * two to a float (a buffer of half as many floats, the lower address in the
+ * low half).  An optional third buffer of pages · key_heads · page floats,
+ * [pages][key_heads][page], sums the attention weight every cached token has
+ * drawn.  A model has one pool per layer; the sequences' pages and lengths
+ * are in a table that all layers use.
+ *
+ * Every buffer and table must belong to the context of the call
+ * (SLM_ERR_INVALID otherwise), no buffer may be passed twice, and a call
+ * made while the context's stream is being captured fails with
+ * SLM_ERR_INVALID.  Calls queue on the context's stream and read the table as
+ * it is when the call is made.                                             */
+/* ---------------------------------------------------------------------- */
+
+/* A table of `seqs` sequences of up to `per_seq` pages of `page` tokens, page
+ * ids below `pages`.  Every sequence starts without pages, at length 0.
+ * Limits: seqs ≤ 65535, per_seq · page < 2^31, pages < 2^31. */
+int slm_table_new(slm_ctx* ctx, size_t seqs, size_t per_seq, size_t page, size_t pages, slm_table** out);
+int slm_table_free(slm_table* table);
+/* Sequence `seq` has the n pages ids[0..n): slot s is row s % page of page
+ * ids[s / page].  An id may not come twice in one sequence.  Two sequences may
+ * list one page (a common beginning); such a page is read, never written (see
+ * the calls below).  Fails when n pages do not hold the sequence's length. */
+int slm_table_assign(slm_table* table, size_t seq, const uint32_t* ids, size_t n);
+/* The lengths of all sequences (n must be seqs): sequence i holds lens[i]
+ * tokens, slots 0 .. lens[i]-1; 0 is an idle row.  Fails, changing nothing,
+ * when a length does not fit the sequence's pages. */
+int slm_table_set_lens(slm_table* table, const uint32_t* lens, size_t n);
+int slm_table_lens(const slm_table* table, uint32_t* out, size_t n);
+
+#define SLM_PAGES_F32 0
+#define SLM_PAGES_BF16 1
+typedef struct slm_paged {
+  size_t heads;     /* query heads (attend only), a multiple of key_heads */
+  size_t key_heads;
+  size_t dh;        /* head size: a multiple of 8, at most 256 */
+  size_t reach;     /* attend: a query sees the last `reach` tokens; SIZE_MAX: all */
+  float scale;      /* attend: factor of the scores */
+  int type;         /* SLM_PAGES_F32 or SLM_PAGES_BF16 */
+} slm_paged;
+
+/* Stores the last m tokens of sequences first .. first+count-1: row j of
+ * sequence i (row (i-first)·m + j of ksrc and vsrc, key_heads · dh floats at
+ * koff + row·ldk and voff + row·ldv) goes to slot lens[i]-m+j; rows whose slot
+ * would be negative (idle rows, a prompt shorter than m) are skipped.  The
+ * table's lengths include the tokens stored.  bf16 pages hold the nearest
+ * value, ties to even.  With `weights` (null: none) the stored tokens' weights
+ * become 0.  Fails when a slot lies in a page that another sequence lists. */
+int slm_op_paged_store(slm_ctx* ctx, slm_buf* k, slm_buf* v, slm_buf* weights, slm_table* table, size_t first,
+                       size_t count, const slm_buf* ksrc, size_t koff, size_t ldk, const slm_buf* vsrc, size_t voff,
+                       size_t ldv, size_t m, const slm_paged* p);
+/* Attention of one query per sequence over its cached tokens: y[i][h] =
+ * Σ_s p_s v_s over visible slots s, p = softmax of scale · q[i][h]·k_s, with
+ * query head h reading key head h / (heads / key_heads).  Row i of q is heads
+ * · dh floats at qoff + i·ldq; y is seqs × heads × dh, grown as needed; an
+ * idle row gives zeros.  `scores` is scratch (resized as needed).  With
+ * `weights` (null: none) every visible token's weight grows by the sum of its
+ * p over the query heads of its key head; fails when two sequences list one
+ * page.  Arithmetic is f32 (page values as stored).  Where a query, or a
+ * visible key or value, is not finite, that sequence's results are not
+ * either or are NaN; slots outside the visible range are not read. */
+int slm_op_paged_attend(slm_ctx* ctx, slm_buf* y, slm_buf* scores, const slm_buf* q, size_t qoff, size_t ldq,
+                        const slm_buf* k, const slm_buf* v, slm_buf* weights, slm_table* table, const slm_paged* p);
+/* Brings every sequence of `from` down to at most `keep` tokens per key head,
+ * writing them to the pages of `to` (a table of the same sequences over the
+ * same pool).  Per sequence and key head: up to `keep` tokens are all kept;
+ * of more, the first `sinks`, the last `recent` (sinks + recent ≤ keep) and
+ * then those of the highest weight (equal weights: the lower slot first; NaN
+ * below every number), in slot order.  K, V and weight rows are copied; the
+ * rows they came from, and the rows of `to`'s pages behind the last kept
+ * token, stay as they were.  kept[i][key head][j] (32-bit words, seqs ×
+ * key_heads × keep, grown as needed) is the slot in `from` that slot j of `to`
+ * came from, 0xFFFFFFFF past the last.  `to`'s lengths become min(length,
+ * keep).  Fails when `to`'s pages do not hold them, are listed twice in `to`,
+ * or are listed in `from`. */
+int slm_op_paged_evict(slm_ctx* ctx, slm_buf* kept, slm_buf* k, slm_buf* v, slm_buf* weights, slm_table* from,
+                       slm_table* to, size_t keep, size_t sinks, size_t recent, const slm_paged* p);
 
 /* ---------------------------------------------------------------------- */
 /* Model level (src/model.rs, src/sample.rs).                              */

@@ -38,6 +38,7 @@ SLM_OPT_MEGA = 2
 SLM_OPT_TRACE = 3
 SLM_OPT_TEST_STALL = 4
 SLM_OPT_BF16 = 5
+SLM_PAGES_F32, SLM_PAGES_BF16 = 0, 1
 SLM_STAT_STEP_KERNELS, SLM_STAT_GRAPHS, SLM_STAT_MEGA, SLM_STAT_PHASES = 1, 2, 3, 4
 SIZE_MAX = (1 << 64) - 1
 
@@ -51,6 +52,10 @@ class SlmError(RuntimeError):
 class _Attn(_c.Structure):
     _fields_ = [(n, _sz) for n in ("pos", "m", "reach", "gap", "cap", "heads", "key_heads", "dh")] + [
         ("scale", _c.c_float)]
+
+
+class _Paged(_c.Structure):
+    _fields_ = [(n, _sz) for n in ("heads", "key_heads", "dh", "reach")] + [("scale", _c.c_float), ("type", _c.c_int)]
 
 
 class _Sampling(_c.Structure):
@@ -105,6 +110,15 @@ _SIGS = {
     "slm_op_store": (_c.c_int, [_vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz]),
     "slm_op_attend": (_c.c_int, [_vp, _vp, _vp, _vp, _sz, _vp, _vp, _c.POINTER(_Attn)]),
     "slm_op_attend_noalloc": (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _c.POINTER(_Attn)]),
+    "slm_table_new": (_c.c_int, [_vp, _sz, _sz, _sz, _sz, _c.POINTER(_vp)]),
+    "slm_table_free": (_c.c_int, [_vp]),
+    "slm_table_assign": (_c.c_int, [_vp, _sz, _u32p, _sz]),
+    "slm_table_set_lens": (_c.c_int, [_vp, _u32p, _sz]),
+    "slm_table_lens": (_c.c_int, [_vp, _u32p, _sz]),
+    "slm_op_paged_store": (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _sz, _sz, _vp, _sz, _sz, _vp, _sz, _sz, _sz,
+                                      _c.POINTER(_Paged)]),
+    "slm_op_paged_attend": (_c.c_int, [_vp, _vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _c.POINTER(_Paged)]),
+    "slm_op_paged_evict": (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _c.POINTER(_Paged)]),
     "slm_model_load": (_c.c_int, [_vp, _c.c_char_p, _c.POINTER(_vp)]),
     "slm_model_free": (_c.c_int, [_vp]),
     "slm_model_info_get": (_c.c_int, [_vp, _c.POINTER(_Info)]),
@@ -288,6 +302,42 @@ class Buf:
         return out
 
 
+class Table:
+    """Pages and lengths of the sequences of a paged key-value cache (slm_table_*): `seqs` sequences
+    of up to `per_seq` pages of `page` tokens, page ids below `pages`."""
+
+    def __init__(self, ctx: Context, seqs: int, per_seq: int, page: int, pages: int):
+        h = _vp()
+        _check(lib().slm_table_new(ctx._h, seqs, per_seq, page, pages, _c.byref(h)))
+        self.ctx, self.seqs, self.per_seq, self.page, self.pages = ctx, seqs, per_seq, page, pages
+        self._h = h
+        self._free = lib().slm_table_free
+
+    def close(self):
+        # The free function is looked up while the module is intact: at
+        # interpreter exit its globals may already be gone.
+        if getattr(self, "_h", None):
+            self._free(self._h)
+            self._h = None
+
+    __del__ = close
+
+    def assign(self, seq: int, ids) -> None:
+        """Sequence `seq` has the pages `ids`: slot s is row s % page of page ids[s // page]."""
+        ids = _u32(ids)
+        _check(lib().slm_table_assign(self._h, seq, ids.ctypes.data_as(_u32p), ids.size))
+
+    def set_lens(self, lens) -> None:
+        """Cached tokens of every sequence (0: idle)."""
+        lens = _u32(lens)
+        _check(lib().slm_table_set_lens(self._h, lens.ctypes.data_as(_u32p), lens.size))
+
+    def lens(self) -> np.ndarray:
+        out = np.empty(self.seqs, dtype=np.uint32)
+        _check(lib().slm_table_lens(self._h, out.ctypes.data_as(_u32p), out.size))
+        return out
+
+
 class Ops:
     """The reference's `Ops` trait (src/ops.rs:68-228) on one context.
 
@@ -392,6 +442,40 @@ class Ops:
         qb, qo = self._at(q)
         a = _Attn(pos, m, SIZE_MAX if reach is None else reach, gap, cap, heads, key_heads, dh, scale)
         _check(lib().slm_op_attend(self._c, y._h, scores._h, qb._h, qo, k._h, v._h, _c.byref(a)))
+
+
+    # Paged key-value caches (slm_op_paged_*; no counterpart in the reference).  k and v are pools of
+    # [pages][key_heads][page][dh] values, f32 or, with bf16=True, bf16 values two to a float; weights
+    # (optional but for paged_evict) is [pages][key_heads][page].
+
+    def paged_store(self, k: Buf, v: Buf, table: Table, ksrc, vsrc, *, m: int, key_heads: int, dh: int,
+                    first: int = 0, count: int | None = None, ldk: int | None = None, ldv: int | None = None,
+                    bf16: bool = False, weights: Buf | None = None) -> None:
+        """The last m tokens of sequences first .. first + count - 1 (count None: all that follow)."""
+        (kb, ko), (vb, vo) = self._at(ksrc), self._at(vsrc)
+        width = key_heads * dh
+        p = _Paged(0, key_heads, dh, 0, 0.0, SLM_PAGES_BF16 if bf16 else SLM_PAGES_F32)
+        _check(lib().slm_op_paged_store(self._c, k._h, v._h, weights._h if weights else None, table._h, first,
+                                        table.seqs - first if count is None else count, kb._h, ko,
+                                        width if ldk is None else ldk, vb._h, vo, width if ldv is None else ldv, m,
+                                        _c.byref(p)))
+
+    def paged_attend(self, y: Buf, scores: Buf, q, k: Buf, v: Buf, table: Table, *, heads: int, key_heads: int,
+                     dh: int, scale: float, reach: int | None = None, ldq: int | None = None, bf16: bool = False,
+                     weights: Buf | None = None) -> None:
+        """One query per sequence; reach None is unbounded; weights grow by what each token draws."""
+        qb, qo = self._at(q)
+        p = _Paged(heads, key_heads, dh, SIZE_MAX if reach is None else reach, scale,
+                   SLM_PAGES_BF16 if bf16 else SLM_PAGES_F32)
+        _check(lib().slm_op_paged_attend(self._c, y._h, scores._h, qb._h, qo, heads * dh if ldq is None else ldq, k._h,
+                                         v._h, weights._h if weights else None, table._h, _c.byref(p)))
+
+    def paged_evict(self, kept: Buf, k: Buf, v: Buf, weights: Buf, src: Table, dst: Table, *, keep: int, sinks: int,
+                    recent: int, key_heads: int, dh: int, bf16: bool = False) -> None:
+        """At most `keep` tokens per sequence and key head, from src's pages to dst's; kept holds 32-bit words."""
+        p = _Paged(0, key_heads, dh, 0, 0.0, SLM_PAGES_BF16 if bf16 else SLM_PAGES_F32)
+        _check(lib().slm_op_paged_evict(self._c, kept._h, k._h, v._h, weights._h, src._h, dst._h, keep, sinks, recent,
+                                        _c.byref(p)))
 
 
 def attend_noalloc(ctx: Context, y: Buf, q: Buf, k: Buf, v: Buf, *, pos: int, m: int, reach: int | None, gap: int,

@@ -1,0 +1,129 @@
+// The host's copy of a paged cache's table: which pages a sequence has, how
+// many tokens, and which sequences list a page.  Plain C++ (no CUDA), so that
+// everything a kernel will index with is checked, and tested, without a GPU.
+// A refused call throws std::invalid_argument and changes nothing.
+#pragma once
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <stdexcept>
+#include <string>
+#include <vector>
+
+namespace slm {
+
+inline void table_require(bool ok, const std::string& msg) {
+  if (!ok) throw std::invalid_argument(msg);
+}
+
+inline size_t checked_mul(size_t a, size_t b) {
+  size_t r;
+  table_require(!__builtin_mul_overflow(a, b, &r), "paged: size overflows");
+  return r;
+}
+
+inline size_t checked_add(size_t a, size_t b) {
+  size_t r;
+  table_require(!__builtin_add_overflow(a, b, &r), "paged: size overflows");
+  return r;
+}
+
+class PageTable {
+ public:
+  PageTable(size_t seqs, size_t per, size_t page, size_t pages) : seqs(seqs), per(per), page(page), pages(pages) {
+    table_require(seqs > 0 && seqs <= 65535, "table: 1 to 65535 sequences");
+    table_require(per > 0 && page > 0 && checked_mul(per, page) < ((size_t)1 << 31), "table: bad pages per sequence");
+    table_require(pages > 0 && pages < ((size_t)1 << 31), "table: bad number of pages");
+    table_require(checked_add(seqs, checked_mul(seqs, per)) < ((size_t)1 << 32), "table: too many pages in all");
+    words.assign(seqs + seqs * per, 0);
+    held.assign(seqs, 0);
+    uses.assign(pages, 0);
+  }
+
+  const size_t seqs, per, page, pages;
+  // lens[seqs], then ids[seqs][per]: the layout the kernels read.
+  std::vector<uint32_t> words;
+  std::vector<uint32_t> held;  // pages of each sequence
+  std::vector<uint32_t> uses;  // sequences that list each page
+  size_t shared = 0;           // pages listed by more than one
+  size_t lo = 0, hi = 0;       // words changed since settle()
+
+  uint32_t len(size_t i) const { return words[i]; }
+  const uint32_t* ids(size_t i) const { return words.data() + seqs + i * per; }
+  void settle() { lo = hi = 0; }
+
+  void assign(size_t seq, const uint32_t* list, size_t n) {
+    table_require(list || n == 0, "table_assign: bad arguments");
+    table_require(seq < seqs, "table_assign: no such sequence");
+    table_require(n <= per, "table_assign: more pages than the table has room for");
+    table_require(len(seq) <= n * page, "table_assign: the pages do not hold the sequence's length");
+    std::vector<uint32_t> sorted(list, list + n);
+    std::sort(sorted.begin(), sorted.end());
+    table_require(n == 0 || sorted.back() < pages, "table_assign: page id out of range");
+    table_require(std::adjacent_find(sorted.begin(), sorted.end()) == sorted.end(),
+                  "table_assign: a page comes twice in one sequence");
+    uint32_t* row = words.data() + seqs + seq * per;
+    for (size_t j = 0; j < held[seq]; j++) shared -= --uses[row[j]] == 1;
+    for (size_t j = 0; j < n; j++) shared += ++uses[list[j]] == 2;
+    size_t same = 0;  // a sequence that grew keeps its first pages
+    while (same < n && same < held[seq] && row[same] == list[same]) same++;
+    std::copy(list + same, list + n, row + same);
+    held[seq] = (uint32_t)n;
+    if (same < n) touch(seqs + seq * per + same, seqs + seq * per + n);
+  }
+
+  void set_lens(const uint32_t* lens, size_t n) {
+    table_require(lens, "table_set_lens: bad arguments");
+    table_require(n == seqs, "table_set_lens: one length per sequence");
+    for (size_t i = 0; i < n; i++)
+      table_require(lens[i] <= held[i] * page, "table_set_lens: sequence " + std::to_string(i) + " has " +
+                                                   std::to_string(held[i]) + " pages, too few for " +
+                                                   std::to_string(lens[i]) + " tokens");
+    for (size_t i = 0; i < n; i++) set_len(i, lens[i]);
+  }
+
+  void set_len(size_t i, uint32_t v) {
+    if (words[i] == v) return;
+    words[i] = v;
+    touch(i, i + 1);
+  }
+
+  // The last m tokens of sequences first .. first + count - 1 may be written.
+  void check_store(size_t first, size_t count, size_t m) const {
+    table_require(first <= seqs && count <= seqs - first, "paged_store: no such sequences");
+    table_require(m < ((size_t)1 << 31), "paged_store: too many tokens");
+    if (!shared || !m) return;
+    for (size_t i = first; i < first + count; i++)
+      for (size_t j = (len(i) > m ? len(i) - m : 0) / page; j * page < len(i); j++)
+        table_require(uses[ids(i)[j]] == 1, "paged_store: a page is listed by two sequences");
+  }
+
+  // At most `keep` tokens of each sequence may move to the pages of `to`.
+  void check_evict(const PageTable& to, size_t keep, size_t sinks, size_t recent) const {
+    table_require(this != &to, "paged_evict: the tables are one");
+    table_require(seqs == to.seqs && page == to.page && pages == to.pages,
+                  "paged_evict: the tables are of different sequences or pools");
+    table_require(keep > 0 && keep < ((size_t)1 << 31), "paged_evict: bad budget");
+    table_require(sinks <= keep && recent <= keep - sinks, "paged_evict: sinks and recent exceed the budget");
+    for (size_t i = 0; i < seqs; i++) {
+      const size_t n = std::min<size_t>(len(i), keep);
+      table_require(n <= to.held[i] * to.page,
+                    "paged_evict: sequence " + std::to_string(i) + " has too few pages to go to");
+      for (size_t j = 0; j * page < n; j++) {
+        const uint32_t id = to.ids(i)[j];
+        table_require(to.uses[id] == 1, "paged_evict: a page to go to is listed by two sequences");
+        table_require(uses[id] == 0, "paged_evict: a page to go to is one that tokens come from");
+      }
+    }
+  }
+
+ private:
+  void touch(size_t a, size_t b) {
+    if (lo == hi) lo = a, hi = b;
+    lo = std::min(lo, a), hi = std::max(hi, b);
+  }
+};
+
+}  // namespace slm

@@ -1,0 +1,64 @@
+// Paged key-value caches: what the host side (paged.cpp) hands the kernels.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace slm {
+
+// A table on the device and the pool's geometry.  Row s of sequence i, key
+// head h is row (ids[i·per + s / page] · key_heads + h) · page + s % page of
+// the pool's K, V ([rows][dh]) and weights ([rows]).
+struct PagedTable {
+  const uint32_t* lens = nullptr;
+  const uint32_t* ids = nullptr;
+  int n = 0, per = 0, page = 0;
+};
+
+struct PagedStoreArgs {
+  PagedTable t;
+  int first, count, m, key_heads, dh;
+  bool bf16;
+  const float *ks, *vs;
+  long long ldk, ldv;
+  void *k, *v;
+  float* weights;  // or null
+};
+void paged_store(const PagedStoreArgs& a, cudaStream_t st);
+
+struct PagedAttendArgs {
+  PagedTable t;
+  const uint32_t* host_lens;  // the lengths the launch is shaped by (the table's)
+  int heads, key_heads, dh;
+  long long reach;  // 0: all
+  float scale;
+  bool bf16;
+  const float* q;
+  long long ldq;
+  const void *k, *v;
+  float* weights;  // or null
+  float* y;
+  float* scratch;
+};
+// Floats of scratch the call needs.
+size_t paged_attend_scratch(const PagedAttendArgs& a);
+void paged_attend(const PagedAttendArgs& a, cudaStream_t st);
+
+struct PagedEvictArgs {
+  PagedTable from, to;
+  int key_heads, dh;
+  bool bf16;
+  int keep, sinks, recent;
+  void *k, *v;
+  float* weights;
+  uint32_t* kept;  // [n][key_heads][keep]
+};
+void paged_evict(const PagedEvictArgs& a, cudaStream_t st);
+
+// words[at[j]] = value[j] for j < n (≤ kPutWords): table updates, by value in
+// the launch parameters, so nothing on the host has to outlive the call.
+constexpr int kPutWords = 480;
+void table_put(uint32_t* words, const uint32_t* at, const uint32_t* value, int n, cudaStream_t st);
+
+}  // namespace slm
