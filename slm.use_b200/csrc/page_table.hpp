@@ -33,8 +33,8 @@ inline size_t checked_add(size_t a, size_t b) {
 class PageTable {
  public:
   PageTable(size_t seqs, size_t per, size_t page, size_t pages) : seqs(seqs), per(per), page(page), pages(pages) {
-    table_require(seqs > 0 && seqs <= 65535, "table: 1 to 65535 sequences");
-    table_require(per > 0 && page > 0 && checked_mul(per, page) < ((size_t)1 << 31), "table: bad pages per sequence");
+    table_require(seqs > 0 && seqs <= 4096, "table: 1 to 4096 sequences");
+    table_require(per > 0 && page > 0 && checked_mul(per, page) < ((size_t)1 << 30), "table: bad pages per sequence");
     table_require(pages > 0 && pages < ((size_t)1 << 31), "table: bad number of pages");
     table_require(checked_add(seqs, checked_mul(seqs, per)) < ((size_t)1 << 32), "table: too many pages in all");
     words.assign(seqs + seqs * per, 0);

@@ -200,6 +200,7 @@ int slm_op_paged_attend(slm_ctx* c, slm_buf* y, slm_buf* scores, const slm_buf* 
     a.k = k->ptr, a.v = v->ptr, a.weights = weights ? weights->ptr : nullptr;
     ensure(y, t->host.seqs * width);
     ensure(scores, paged_attend_scratch(a));
+    a.counters = merge_counters(c, paged_attend_counters(a));
     a.y = y->ptr, a.scratch = scores->ptr;
     flush(t);
     paged_attend(a, c->stream);

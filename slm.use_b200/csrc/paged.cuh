@@ -39,10 +39,13 @@ struct PagedAttendArgs {
   const void *k, *v;
   float* weights;  // or null
   float* y;
-  float* scratch;
+  float* scratch;      // paged_attend_scratch(a) floats, 16-byte aligned
+  unsigned* counters;  // paged_attend_counters(a) words, zero between launches
 };
-// Floats of scratch the call needs.
+// Shared-memory limits of the kernels, once per device.
+void paged_prepare();
 size_t paged_attend_scratch(const PagedAttendArgs& a);
+size_t paged_attend_counters(const PagedAttendArgs& a);
 void paged_attend(const PagedAttendArgs& a, cudaStream_t st);
 
 struct PagedEvictArgs {

@@ -12,6 +12,7 @@
 #include "capi.hpp"
 #include "common.cuh"
 #include "kernels.cuh"
+#include "paged.cuh"
 
 namespace slm {
 
@@ -81,6 +82,18 @@ void* stage(slm_ctx* c, const void* host, size_t bytes) {
   // Pageable source: the runtime copies it before returning, so `host` may go.
   SLM_CUDA(cudaMemcpyAsync(c->stage, host, bytes, cudaMemcpyHostToDevice, c->stream));
   return c->stage;
+}
+
+unsigned* merge_counters(slm_ctx* c, size_t n) {
+  if (c->merge_cnt_len < n) {
+    SLM_CUDA(cudaStreamSynchronize(c->stream));
+    dev_free(c->merge_cnt);
+    c->merge_cnt = nullptr, c->merge_cnt_len = 0;
+    c->merge_cnt = static_cast<unsigned*>(dev_alloc(n * sizeof(unsigned)));
+    SLM_CUDA(cudaMemsetAsync(c->merge_cnt, 0, n * sizeof(unsigned), c->stream));
+    c->merge_cnt_len = n;
+  }
+  return c->merge_cnt;
 }
 
 void gemm_workspace(slm_ctx* c, LinearArgs& a, bool capturing) {
@@ -170,6 +183,7 @@ int slm_ctx_new(int device, slm_ctx** out) {
       Device dev(c);
       SLM_CUDA(cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking));
       linear_prepare();
+      paged_prepare();
       c->err = static_cast<int*>(dev_alloc(sizeof(int) * 4));
       SLM_CUDA(cudaMemsetAsync(c->err, 0, sizeof(int) * 4, c->stream));
       SLM_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&c->err_host), sizeof(int) * 4, cudaHostAllocDefault));
@@ -535,17 +549,9 @@ int slm_op_attend(slm_ctx* c, slm_buf* y, slm_buf* scores, const slm_buf* q, siz
       qs = scores->ptr + qat;
     }
     // Counters for merging the slices in the slice launch (kept zero between calls).
-    const size_t ncnt = at->m * at->heads;
-    if (c->merge_cnt_len < ncnt) {
-      SLM_CUDA(cudaStreamSynchronize(c->stream));
-      dev_free(c->merge_cnt);
-      c->merge_cnt = nullptr, c->merge_cnt_len = 0;
-      c->merge_cnt = static_cast<unsigned*>(dev_alloc(ncnt * sizeof(unsigned)));
-      SLM_CUDA(cudaMemsetAsync(c->merge_cnt, 0, ncnt * sizeof(unsigned), c->stream));
-      c->merge_cnt_len = ncnt;
-    }
+    unsigned* cnt = merge_counters(c, at->m * at->heads);
     attention(qs, (int)(at->heads * at->dh), k->ptr, v->ptr, g, nullptr, nsplit, scores->ptr + 2, y->ptr,
-              (int)(at->heads * at->dh), c->stream, c->merge_cnt);
+              (int)(at->heads * at->dh), c->stream, cnt);
   });
 }
 

@@ -511,6 +511,8 @@ def test_two_contexts_at_once(slm, ctx, ops):
 
 
 def test_refusals(slm, ctx, ops):
+    import gc
+
     import torch
     rng = np.random.default_rng(42)
     pool = Pool(slm, ctx, ops, rng, [20, 3], 2, 64, 16, False)
@@ -567,11 +569,16 @@ def test_refusals(slm, ctx, ops):
     x += 1  # its kernel is loaded before the capture
     x.zero_()
     torch.cuda.synchronize()
-    with torch.cuda.graph(g, stream=stream, capture_error_mode="thread_local"):
-        x += 1
-        refused(attend)
-        refused(ops.paged_store, pool.kb, pool.vb, pool.table, src, src, **put)
-        refused(ops.paged_evict, kept, pool.kb, pool.vb, pool.wb, pool.table, to, **cut)
+    gc.collect()
+    gc.disable()  # a buffer freed during the capture would wait for the stream
+    try:
+        with torch.cuda.graph(g, stream=stream, capture_error_mode="thread_local"):
+            x += 1
+            refused(attend)
+            refused(ops.paged_store, pool.kb, pool.vb, pool.table, src, src, **put)
+            refused(ops.paged_evict, kept, pool.kb, pool.vb, pool.wb, pool.table, to, **cut)
+    finally:
+        gc.enable()
     g.replay()
     torch.cuda.synchronize()
     assert x.tolist() == [1.0] * 8

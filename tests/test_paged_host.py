@@ -84,9 +84,9 @@ def table(host):
         host.pt_free(t.h)
 
 
-@pytest.mark.parametrize("shape", [(0, 1, 1, 1), (65536, 1, 1, 1), (1, 0, 1, 1), (1, 1, 0, 1), (1, 1, 1, 0),
+@pytest.mark.parametrize("shape", [(0, 1, 1, 1), (4097, 1, 1, 1), (1, 0, 1, 1), (1, 1, 0, 1), (1, 1, 1, 0),
                                    (1, 1 << 16, 1 << 15, 4), (1, 2, (1 << 64) - 1, 4), (2, (1 << 64) - 1, 1, 4),
-                                   (1, 1, 1, 1 << 31), (65535, 1 << 17, 1, 4)])
+                                   (1, 1, 1, 1 << 31), (4096, 1 << 20, 1, 4)])
 def test_impossible_tables_are_refused(host, shape):
     with pytest.raises(ValueError):
         HostTable(host, *shape)
