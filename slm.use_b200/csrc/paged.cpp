@@ -45,7 +45,8 @@ void flush(slm_table* t) {
 PagedTable on_device(slm_table* t) {
   PagedTable d;
   d.lens = t->dev, d.ids = t->dev + t->host.seqs;
-  d.n = (int)t->host.seqs, d.per = (int)t->host.per, d.page = (int)t->host.page;
+  d.n = (int)t->host.seqs, d.per = (int)t->host.per;
+  d.set_page((uint32_t)t->host.page);
   return d;
 }
 
@@ -73,6 +74,7 @@ void pool(const slm_paged* p, const slm_table* t, const slm_buf* k, const slm_bu
   SLM_REQUIRE(p->dh >= 8 && p->dh <= 256 && p->dh % 8 == 0, w + ": head size must be a multiple of 8, at most 256");
   SLM_REQUIRE(p->key_heads > 0 && p->key_heads <= 65535, w + ": bad number of key heads");
   const size_t rows = checked_mul(checked_mul(t->host.pages, p->key_heads), t->host.page);
+  SLM_REQUIRE(rows < ((size_t)1 << 32), w + ": pages x key heads x page must stay below 2^32");
   const size_t floats = p->type == SLM_PAGES_BF16 ? checked_mul(rows, p->dh / 2) : checked_mul(rows, p->dh);
   view(k, 0, floats, (w + " k").c_str());
   view(v, 0, floats, (w + " v").c_str());
@@ -200,7 +202,6 @@ int slm_op_paged_attend(slm_ctx* c, slm_buf* y, slm_buf* scores, const slm_buf* 
     a.k = k->ptr, a.v = v->ptr, a.weights = weights ? weights->ptr : nullptr;
     ensure(y, t->host.seqs * width);
     ensure(scores, paged_attend_scratch(a));
-    a.counters = merge_counters(c, paged_attend_counters(a));
     a.y = y->ptr, a.scratch = scores->ptr;
     flush(t);
     paged_attend(a, c->stream);

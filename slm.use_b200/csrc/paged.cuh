@@ -13,7 +13,19 @@ namespace slm {
 struct PagedTable {
   const uint32_t* lens = nullptr;
   const uint32_t* ids = nullptr;
-  int n = 0, per = 0, page = 0;
+  int n = 0, per = 0;
+  uint32_t page = 0;
+  // page_of(s) = s / page for s < 2^30: s · mul >> shift with mul =
+  // ⌈2^(30+k) / page⌉, k = ⌈log2 page⌉ (mul · page - 2^(30+k) < 2^k, so the
+  // quotient's error stays below 1 / page).
+  uint32_t mul = 0, shift = 0;
+  void set_page(uint32_t p) {
+    uint32_t k = 0;
+    while ((1u << k) < p) k++;
+    page = p, shift = 30 + k;
+    mul = (uint32_t)((((uint64_t)1 << shift) + p - 1) / p);
+  }
+  __host__ __device__ uint32_t page_of(uint32_t s) const { return (uint32_t)((uint64_t)s * mul >> shift); }
 };
 
 struct PagedStoreArgs {
@@ -39,13 +51,11 @@ struct PagedAttendArgs {
   const void *k, *v;
   float* weights;  // or null
   float* y;
-  float* scratch;      // paged_attend_scratch(a) floats, 16-byte aligned
-  unsigned* counters;  // paged_attend_counters(a) words, zero between launches
+  float* scratch;  // paged_attend_scratch(a) floats, 16-byte aligned
 };
 // Shared-memory limits of the kernels, once per device.
 void paged_prepare();
 size_t paged_attend_scratch(const PagedAttendArgs& a);
-size_t paged_attend_counters(const PagedAttendArgs& a);
 void paged_attend(const PagedAttendArgs& a, cudaStream_t st);
 
 struct PagedEvictArgs {

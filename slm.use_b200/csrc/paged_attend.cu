@@ -7,10 +7,12 @@
 // Keys and values are read once, so bytes bound the call; the rest is arranged
 // to stay under them.
 //
-// Work: the visible slots of a (sequence, tile of up to 8 query heads of one
-// key head) are cut into chunks of equal length, one CTA each (4 warps, every
-// warp its own tiles of the chunk); the last CTA of a cut (sequence, tile)
-// joins the chunks' partials in order, so results do not depend on timing.
+// Work: the visible slots of every pair, a (sequence, tile of up to 8 query
+// heads of one key head), lie one after the other and are shared evenly over
+// all warps that fit on the GPU at once, whatever the sequences' lengths; a
+// warp works alone, and a second kernel joins the pieces of cut pairs in order,
+// so results do not depend on timing.  Where all pairs are short, a CTA's four
+// warps share one and join it themselves.
 //
 // Data: a warp streams its tiles through three private buffers with 16-byte
 // asynchronous copies, which look every row's page up (a page may end
@@ -36,39 +38,56 @@ namespace slm {
 
 namespace {
 
-constexpr int kWarps = 4, kThreads = kWarps * 32, kHeads = 8, kStages = 3;
+constexpr int kWarps = 4, kThreads = kWarps * 32, kHeads = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.0f;     // scores (log2 units) may exceed m by this before m moves
-constexpr int kMaxChunks = 1024;  // chunks of one sequence
 constexpr int kWeightKeys = 256;  // slots of a CTA of k_paged_weights
 
-// Where a launch keeps what its CTAs hand one another.
+// Where a launch keeps what its warps hand one another.
 struct Scratch {
-  float* part;       // [CTA][heads][dh] sums, then [CTA][heads][2] (m, l), of cut sequences
-  float* part_ml;
-  float* stat;       // [n][heads][2]: final m and 1 / l
+  float* part;       // [warp][2][kHeads][dh]: sums of pieces of cut (sequence, tile)s
+  float* part_ml;    // [warp][2][kHeads][2]: their m and l
+  float* stat;       // [n][heads][2]: final m and 1 / l, or null
   float* score;      // per sequence [heads][visible rounded up to 4], log2 units; or null
-  unsigned* cnt;     // [n][tiles] arrivals, zero between launches
 };
+
+// The lengths travel in the launch parameters where they fit (a CTA then finds
+// its place without waiting for memory), else the table's are read.
+constexpr int kLens = 512;
+struct Lens {
+  uint32_t v[kLens];
+};
+__device__ __forceinline__ uint32_t len_of(const PagedTable& t, const Lens& lens, int i) {
+  return t.n <= kLens ? lens.v[i] : t.lens[i];
+}
 
 __host__ __device__ inline int visible_of(uint32_t len, long long reach) {
   return reach && (long long)len > reach ? (int)reach : (int)len;
 }
 
-// Tile shape for pages of `size`-byte values and head sizes up to DH: K and V
-// of a tile take 8 KB (16 KB at f32, 256).
+// Slots of a warp's tile, its buffers, and CTAs an SM, for pages of f32 and of
+// bf16 and head sizes up to 64, 128, 256: K and V of a tile take 8 KB (16 KB
+// at 256).  Measured against 3 CTAs an SM with smaller tiles (us, 64 ragged
+// sequences f32 64 / 48 bf16 128 / 8 x 65536 bf16 128): 45.5 / 167 / 319 so,
+// 44.9 / 178 / 341 with two buffers, 46.1 / 204 / 390 with 8-slot tiles.
+constexpr int kCfg[6][3] = {{16, 3, 2}, {8, 3, 2}, {8, 2, 1}, {32, 3, 2}, {16, 3, 2}, {16, 2, 1}};
 template <int SIZE, int DH>
 struct Shape {
+  static constexpr int kIndex = (SIZE == 2 ? 3 : 0) + (DH == 64 ? 0 : DH == 128 ? 1 : 2);
   static constexpr int kRow = DH * SIZE;             // bytes of a row in shared memory
-  static constexpr int kKeys = 4096 / kRow < 8 ? 8 : 4096 / kRow;
+  static constexpr int kKeys = kCfg[kIndex][0];
+  static constexpr int kStages = kCfg[kIndex][1];
   static constexpr int kTile = kKeys * kRow;         // K (or V) bytes of a tile
-  static constexpr int kBuffers = kWarps * kStages * 2 * kTile;
   static constexpr bool kQShared = DH > 128;         // q in shared memory: registers hold the sums
-  static constexpr int kQ = kQShared ? DH / 8 * 512 : 0;
-  static constexpr int kSmem = kBuffers + kQ;
-  static constexpr int kCtas = kSmem <= 113 * 1024 ? 2 : 1;
+  static constexpr int kWarp = kStages * 2 * kTile + (kQShared ? DH / 8 * 512 : 0);  // bytes of a warp
+  static constexpr int kSmem = kWarps * kWarp;
+  static constexpr int kCtas = kCfg[kIndex][2];
 };
 
+__device__ __forceinline__ void copy16(uint32_t dst, const char* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// 16 bytes, or zeros and no read.
 __device__ __forceinline__ void copy16(uint32_t dst, const char* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
@@ -90,6 +109,12 @@ __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, ui
       "%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ float exp2_of(float x) {  // relative error 2^-22; 0 below 2^-126
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // The upper 11 significant bits of x, and the rest (read by the tensor core to
@@ -120,393 +145,554 @@ struct Operand<true> {
   static __device__ __forceinline__ void mul(float* c, const uint32_t* a, uint32_t x0, uint32_t x1) { mma(c, a, x0, x1); }
 };
 
-// The sequence and chunk of CTA-row `at`: sequences' chunks lie one after the
-// other.  Also the rounded visible slots of the sequences before it.
-struct Place {
-  int seq, chunk, chunks, visible;
-  long long before;
-};
-__device__ Place find_place(const PagedTable& t, long long reach, int keys, int at) {
-  __shared__ int s_chunks[kThreads / 32];
-  __shared__ long long s_slots[kThreads / 32];
-  __shared__ Place s_place;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
-  const int each = (t.n + blockDim.x - 1) / blockDim.x;
-  int mine = 0;
-  long long slots = 0;
-  for (int j = 0; j < each; j++) {
-    const int i = tid * each + j;
-    const int v = i < t.n ? visible_of(t.lens[i], reach) : 0;
-    mine += (v + keys - 1) / keys, slots += (v + 3) & ~3;
+// How a launch's work is laid out.  Every pair, a (sequence, tile of up to 8
+// query heads of one key head), has ⌈visible / keys⌉ blocks of `keys` slots.
+// Pairs lie one after the other in units: `extra` (what beginning a pair costs,
+// in blocks) plus its blocks; with whole = true a pair is one unit, never cut.
+struct Work {
+  uint32_t keys, extra, units;  // units: in all
+  uint32_t takers;              // warps (CTAs if whole) that share them
+  int tiles;                    // pairs of a sequence
+  bool whole;
+  __host__ __device__ uint32_t blocks_of(uint32_t visible) const { return (visible + keys - 1) / keys; }
+  __host__ __device__ uint32_t units_of(uint32_t visible) const {  // of a pair
+    return visible == 0 ? 0 : whole ? 1 : blocks_of(visible) + extra;
   }
-  int upto = mine;
+  // Units are shared evenly: taker w has those from first_unit(w) on; taker_of
+  // is its inverse.
+  __device__ uint32_t first_unit(uint32_t w) const { return (uint32_t)((uint64_t)w * units / takers); }
+  __device__ uint32_t taker_of(uint32_t unit) const {
+    return (uint32_t)((((uint64_t)unit + 1) * takers - 1) / units);
+  }
+};
+
+// Finds the sequence that holds unit `at` (every warp for itself) and what lies
+// before it.
+struct Place {
+  int seq, visible;
+  uint32_t unit;       // at, counted from the sequence's first unit
+  long long slots;     // visible slots of the sequences before it, each rounded up to 4
+};
+__device__ __forceinline__ Place locate(const PagedTable& t, const Lens& lens, long long reach, const Work& wk,
+                                        uint32_t at) {
+  const int lane = threadIdx.x & 31, each = (t.n + 31) / 32;
+  uint32_t mine = 0;
+  long long slots = 0;
+#pragma unroll 4
+  for (int j = 0; j < each; j++) {
+    const int i = lane * each + j;
+    const uint32_t v = i < t.n ? visible_of(len_of(t, lens, i), reach) : 0;
+    mine += wk.units_of(v) * wk.tiles, slots += (v + 3) & ~3u;
+  }
+  uint32_t upto = mine;
   long long slots_upto = slots;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int a = __shfl_up_sync(0xffffffffu, upto, o);
+    const uint32_t a = __shfl_up_sync(0xffffffffu, upto, o);
     const long long b = __shfl_up_sync(0xffffffffu, slots_upto, o);
     if (lane >= o) upto += a, slots_upto += b;
   }
-  if (lane == 31) s_chunks[warp] = upto, s_slots[warp] = slots_upto;
-  __syncthreads();
-  for (int w = 0; w < nw; w++)
-    if (w < warp) upto += s_chunks[w], slots_upto += s_slots[w];
-  if (at < upto && at >= upto - mine) {
-    int c = at - (upto - mine);
-    long long b = slots_upto - slots;
-    for (int j = 0;; j++) {
-      const int v = visible_of(t.lens[tid * each + j], reach), n = (v + keys - 1) / keys;
-      if (c < n) {
-        s_place = Place{tid * each + j, c, n, v, b};
-        break;
-      }
-      c -= n, b += (v + 3) & ~3;
-    }
+  const int src = __ffs(__ballot_sync(0xffffffffu, upto > at)) - 1;
+  Place p{src * each, 0, at - __shfl_sync(0xffffffffu, upto - mine, src),
+          __shfl_sync(0xffffffffu, slots_upto - slots, src)};
+  for (;; p.seq++) {
+    p.visible = visible_of(len_of(t, lens, p.seq), reach);
+    const uint32_t n = wk.units_of(p.visible) * wk.tiles;
+    if (p.unit < n) return p;
+    p.unit -= n, p.slots += (p.visible + 3) & ~3;
   }
-  __syncthreads();
-  return s_place;
 }
+
+// A kernel may begin while the one before it in the stream still runs: what
+// follows `wait` sees all that the earlier one wrote.
+__device__ __forceinline__ void dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 template <bool BF16, int DH>
 __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
-    k_paged_attend(PagedAttendArgs a, Scratch sc, int keys, int tiles) {
+    k_paged_attend(const __grid_constant__ PagedAttendArgs a, const __grid_constant__ Scratch sc,
+                   const __grid_constant__ Lens lens, const __grid_constant__ Work wk, bool idle, bool q16) {
   constexpr int SIZE = BF16 ? 2 : 4;
   using S = Shape<SIZE, DH>;
   constexpr int kSteps = DH / 8;            // k-steps of q·k, and 8-column tiles of p·v
   constexpr int kLoad = BF16 ? 4 : 2;       // k-steps that a 16-byte piece of a key row feeds
   constexpr int kPieces = S::kRow / 16;     // 16-byte pieces of a row
+  constexpr int kKeys = S::kKeys, kStages = S::kStages;
+  constexpr int kSum = DH + 4;               // floats of a head's sums in shared memory
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float s_m[kWarps][kHeads], s_l[kWarps][kHeads];
-  __shared__ int s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int tile = blockIdx.x % tiles;
-  const Place at = find_place(a.t, a.reach, keys, blockIdx.x / tiles);
   const int group = a.heads / a.key_heads, per_key = (group + kHeads - 1) / kHeads;
-  const int kh = tile / per_key, head0 = kh * group + (tile % per_key) * kHeads;
-  const int heads = min(kHeads, (kh + 1) * group - head0);
-  const int lo = (int)a.t.lens[at.seq] - at.visible;
-  const int first = lo + at.chunk * keys, end = lo + min(at.visible, (at.chunk + 1) * keys);
-
-  // q, scaled to log2 units and split, in the order the key rows are read:
-  // rows g and g + 8 of the left operand are head g's hi and lo parts.
-  uint32_t qa[S::kQShared ? 1 : kSteps][4];
-  const uint32_t buffers = (uint32_t)__cvta_generic_to_shared(smem);
-  const uint32_t q_shared = buffers + S::kBuffers;
-  {
-    const float* q = a.q + at.seq * a.ldq + (size_t)(head0 + g) * a.dh;
-    const float scale = a.scale * kLog2e;
-#pragma unroll
-    for (int s = 0; s < kSteps; s++) {
-      const int d = (s / kLoad) * (BF16 ? 32 : 16) + t * (BF16 ? 8 : 4) + s % kLoad * 2;
-      const bool ok = g < heads && d < a.dh;  // dh is even
-      uint32_t w[4];
-      split(ok ? q[d] * scale : 0.0f, w[0], w[1]);
-      split(ok ? q[d + 1] * scale : 0.0f, w[2], w[3]);
-      if (S::kQShared) {
-        if (s % kWarps == warp)
-          *reinterpret_cast<uint4*>(smem + S::kBuffers + s * 512 + lane * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++) qa[S::kQShared ? 0 : s][j] = w[j];
-      }
-    }
-    if (S::kQShared) __syncthreads();
-  }
-
-  // This warp's tiles: warp, warp + kWarps, … of the chunk.
-  const uint32_t mine = buffers + warp * (kStages * 2 * S::kTile);
-  const uint32_t* ids = a.t.ids + (size_t)at.seq * a.t.per;
+  const uint32_t mine = (uint32_t)__cvta_generic_to_shared(smem) + warp * S::kWarp;
+  unsigned char* q_shared = smem + warp * S::kWarp + kStages * 2 * S::kTile;
+  const uint32_t q_at = (uint32_t)__cvta_generic_to_shared(q_shared) + lane * 16;
   const char *K = static_cast<const char*>(a.k), *V = static_cast<const char*>(a.v);
   const int row_bytes = a.dh * SIZE, pieces = row_bytes / 16;
-  const int n_tiles = first + warp * S::kKeys < end
-                          ? (end - first - warp * S::kKeys + kWarps * S::kKeys - 1) / (kWarps * S::kKeys)
-                          : 0;
-  auto key_of = [&](int j) { return first + (j * kWarps + warp) * S::kKeys; };
-  // Byte offset in the pool of the row that this lane looks up for tile j.
-  auto look_up = [&](int j) -> long long {
-    const int s = min(key_of(j) + lane % S::kKeys, end - 1);
-    const int page = s / a.t.page;
-    return (((long long)ids[page] * a.key_heads + kh) * a.t.page + (s - page * a.t.page)) * row_bytes;
-  };
-  auto load = [&](int j, long long off) {
-    const uint32_t to = mine + j % kStages * (2 * S::kTile);
-    const int n = end - key_of(j);
+
+  dependents_launch();
+  if (idle)  // rows of idle sequences: zeros
+    for (int i = blockIdx.x; i < a.t.n; i += gridDim.x)
+      if (len_of(a.t, lens, i) == 0)
+        for (int e = threadIdx.x; e < a.heads * a.dh; e += kThreads) a.y[(size_t)i * a.heads * a.dh + e] = 0.0f;
+  // This taker's units, and where they begin.  Where pairs are whole, a CTA's
+  // warps share them block by block; else every warp is a taker of its own.
+  const uint32_t w = wk.whole ? blockIdx.x : blockIdx.x * kWarps + warp;
+  if (w >= wk.takers) return;
+  const int turn = wk.whole ? warp : 0, turns = wk.whole ? kWarps : 1;
+  const uint32_t begin = wk.first_unit(w);
+  uint32_t left = wk.first_unit(w + 1) - begin;
+  Place at = locate(a.t, lens, a.reach, wk, begin);
+
+  while (left) {
+    // A segment: blocks b0 .. b1-1 of the pair's n_blocks.
+    const uint32_t n_blocks = wk.blocks_of(at.visible), n_units = wk.units_of(at.visible);
+    const int tile = at.unit / n_units;
+    const uint32_t u0 = at.unit - tile * n_units, u1 = min(n_units, u0 + left), skip = wk.extra;
+    const uint32_t b0 = u0 > skip ? u0 - skip : 0, b1 = wk.whole ? n_blocks : u1 > skip ? u1 - skip : 0;
+    left -= u1 - u0;
+    at.unit += u1 - u0;
+    if (b0 < b1) {
+    const int kh = tile / per_key, head0 = kh * group + (tile % per_key) * kHeads;
+    const int heads = min(kHeads, (kh + 1) * group - head0);
+    const int lo = (int)len_of(a.t, lens, at.seq) - at.visible;
+    const int first = lo + b0 * kKeys, end = lo + min((uint32_t)at.visible, b1 * kKeys);
+    const uint32_t* ids = a.t.ids + (size_t)at.seq * a.t.per;
+    const int n_tiles = ((int)(b1 - b0) - turn + turns - 1) / turns;  // this warp's blocks
+    auto key_of = [&](int j) { return first + (j * turns + turn) * kKeys; };
+
+    // The pool row that this lane looks up for tile j.
+    auto look_up = [&](int j) -> uint32_t {
+      const uint32_t s = min(key_of(j) + lane % kKeys, end - 1);
+      const uint32_t page = a.t.page_of(s);
+      return (ids[page] * a.key_heads + kh) * a.t.page + (s - page * a.t.page);
+    };
+    auto load = [&](int buffer, int n, uint32_t row) {  // n slots
+      const uint32_t to = mine + buffer * (2 * S::kTile);
+      const bool whole = n >= kKeys && row_bytes == S::kRow;
 #pragma unroll
-    for (int u = 0; u < S::kKeys * kPieces / 32; u++) {
-      const int r = (u * 32 + lane) / kPieces, c = (u * 32 + lane) % kPieces;
-      const long long o = __shfl_sync(0xffffffffu, off, r);
-      const bool ok = r < n && c < pieces;
-      const long long from = ok ? o + c * 16 : 0;
-      // Swizzles under which the reads below hit every bank once.
-      copy16(to + r * S::kRow + ((c ^ ((r & 1) << 2)) << 4), K + from, ok);
-      copy16(to + S::kTile + r * S::kRow + ((c ^ (r & 6)) << 4), V + from, ok);
+      for (int u = 0; u < kKeys * kPieces / 32; u++) {
+        const int r = (u * 32 + lane) / kPieces, c = (u * 32 + lane) % kPieces;
+        const uint64_t from = (uint64_t)__shfl_sync(0xffffffffu, row, r) * (uint32_t)row_bytes + c * 16;
+        // Swizzles under which the reads below hit every bank once.
+        const uint32_t kd = to + r * S::kRow + ((c ^ ((r & 1) << 2)) << 4);
+        const uint32_t vd = to + S::kTile + r * S::kRow + ((c ^ (r & 6)) << 4);
+        if (whole) {
+          copy16(kd, K + from);
+          copy16(vd, V + from);
+        } else {
+          const bool ok = r < n && c < pieces;
+          copy16(kd, ok ? K + from : K, ok);
+          copy16(vd, ok ? V + from : V, ok);
+        }
+      }
+    };
+
+    uint32_t row[kStages - 1];
+#pragma unroll
+    for (int j = 0; j < kStages - 1; j++) row[j] = j < n_tiles ? look_up(j) : 0;
+    // q, scaled to log2 units and split, in the order the key rows are read:
+    // rows g and g + 8 of the left operand are head g's hi and lo parts.
+    uint32_t qa[S::kQShared ? 1 : kSteps][4];
+    {
+      const float* q = a.q + at.seq * a.ldq + (size_t)(head0 + g) * a.dh;
+      float qr[S::kQShared ? 1 : kSteps / kLoad][kLoad * 2];
+      auto read = [&](int i, float* v) {
+        const int d = i * (kLoad * 8) + t * (kLoad * 2);
+        const bool ok = g < heads && d < a.dh;  // dh is a multiple of 8
+#pragma unroll
+        for (int e = 0; e < kLoad * 2; e += 4) {
+          float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (ok && q16)
+            x = *reinterpret_cast<const float4*>(q + d + e);
+          else if (ok)
+            x = make_float4(q[d + e], q[d + e + 1], q[d + e + 2], q[d + e + 3]);
+          v[e] = x.x, v[e + 1] = x.y, v[e + 2] = x.z, v[e + 3] = x.w;
+        }
+      };
+      auto parts = [&](const float* v, int e, uint32_t* to) {
+        split(v[2 * e] * (a.scale * kLog2e), to[0], to[1]);
+        split(v[2 * e + 1] * (a.scale * kLog2e), to[2], to[3]);
+      };
+      if (S::kQShared) {
+#pragma unroll 4
+        for (int i = 0; i < kSteps / kLoad; i++) {
+          float v[kLoad * 2];
+          read(i, v);
+#pragma unroll
+          for (int e = 0; e < kLoad; e++) {
+            uint32_t to[4];
+            parts(v, e, to);
+            *reinterpret_cast<uint4*>(q_shared + (i * kLoad + e) * 512 + lane * 16) =
+                make_uint4(to[0], to[1], to[2], to[3]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kSteps / kLoad; i++) read(i, qr[S::kQShared ? 0 : i]);
+      }
+#pragma unroll
+      for (int j = 0; j < kStages - 1; j++) {
+        if (j < n_tiles) load(j, end - key_of(j), row[j]);
+        copies_commit();
+      }
+      if (kStages - 1 < n_tiles) row[0] = look_up(kStages - 1);
+      if (!S::kQShared) {
+#pragma unroll
+        for (int i = 0; i < kSteps / kLoad; i++)
+#pragma unroll
+          for (int e = 0; e < kLoad; e++)
+            parts(qr[S::kQShared ? 0 : i], e, qa[S::kQShared ? 0 : i * kLoad + e]);
+      }
     }
-  };
 
-  float m = -INFINITY, l = 0.0f, o[kSteps][4];
+    float m = -INFINITY, l = 0.0f, o[kSteps][4];
 #pragma unroll
-  for (int s = 0; s < kSteps; s++)
+    for (int s = 0; s < kSteps; s++)
 #pragma unroll
-    for (int j = 0; j < 4; j++) o[s][j] = 0.0f;
-  float* score = sc.score ? sc.score + at.before * a.heads + (size_t)(head0 + g) * ((at.visible + 3) & ~3) - lo : nullptr;
+      for (int j = 0; j < 4; j++) o[s][j] = 0.0f;
+    float* score = sc.score && g < heads
+                       ? sc.score + at.slots * a.heads + (size_t)(head0 + g) * ((at.visible + 3) & ~3) - lo
+                       : nullptr;
 
-  long long off = 0;
-#pragma unroll
-  for (int j = 0; j < kStages - 1; j++) {
-    if (j < n_tiles) load(j, look_up(j));
-    copies_commit();
-  }
-  if (kStages - 1 < n_tiles) off = look_up(kStages - 1);
-  for (int j = 0; j < n_tiles; j++) {
-    copies_wait<kStages - 2>();
-    __syncwarp();  // every lane's copies of tile j have landed, and all are done with tile j - 1
-    if (j + kStages - 1 < n_tiles) load(j + kStages - 1, off);
-    copies_commit();
-    if (j + kStages < n_tiles) off = look_up(j + kStages);
+    int in = kStages - 1, out = 0;  // buffers
+#pragma unroll 1
+    for (int j = 0; j < n_tiles; j++) {
+      copies_wait<kStages - 2>();
+      __syncwarp();  // every lane's copies of this tile have landed, and all are done with the last one
+      if (j + kStages - 1 < n_tiles) load(in, end - key_of(j + kStages - 1), row[0]);
+      copies_commit();
+      if (j + kStages < n_tiles) row[0] = look_up(j + kStages);
+      in = in + 1 == kStages ? 0 : in + 1;
 
-    const uint32_t kt = mine + j % kStages * (2 * S::kTile), vt = kt + S::kTile;
-    const int key0 = key_of(j);
-    constexpr int kBlocks = S::kKeys / 8;
-    float x[kBlocks][2];
+      const uint32_t kt = mine + out * (2 * S::kTile), vt = kt + S::kTile;
+      out = out + 1 == kStages ? 0 : out + 1;
+      const int key0 = key_of(j);
+      constexpr int kBlocks = kKeys / 8;
+      constexpr int kChains = 2;  // independent sums, so that products overlap
+      float x[kBlocks][2], c[kBlocks][kChains][4];
 #pragma unroll
-    for (int b = 0; b < kBlocks; b++) {
-      constexpr int kChains = 4;  // independent sums, so that products overlap
-      float c[kChains][4];
+      for (int b = 0; b < kBlocks; b++)
 #pragma unroll
-      for (int e = 0; e < kChains; e++) c[e][0] = c[e][1] = c[e][2] = c[e][3] = 0.0f;
-      const uint32_t row = kt + (b * 8 + g) * S::kRow + t * 16;
+        for (int e = 0; e < kChains; e++) c[b][e][0] = c[b][e][1] = c[b][e][2] = c[b][e][3] = 0.0f;
+      const uint32_t krow = kt + g * S::kRow + t * 16;
       const int odd = (g & 1) * 64;
 #pragma unroll
       for (int i = 0; i < kSteps / kLoad; i++) {
-        const uint4 w = lds16(row + i * 64 + (i & 1 ? -odd : odd));
-        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+        uint4 kw[kBlocks];
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++) kw[b] = lds16(krow + b * 8 * S::kRow + i * 64 + (i & 1 ? -odd : odd));
 #pragma unroll
         for (int e = 0; e < kLoad; e++) {
           const int s = i * kLoad + e;
           uint32_t qs[4];
           if (S::kQShared) {
-            const uint4 qw = lds16(q_shared + s * 512 + lane * 16);
+            const uint4 qw = lds16(q_at + s * 512);
             qs[0] = qw.x, qs[1] = qw.y, qs[2] = qw.z, qs[3] = qw.w;
           }
           const uint32_t* qv = S::kQShared ? qs : qa[S::kQShared ? 0 : s];
-          if (BF16)
-            Operand<BF16>::mul(c[s % kChains], qv, v[e] << 16, v[e] & 0xffff0000u);
-          else
-            Operand<BF16>::mul(c[s % kChains], qv, v[e * 2], v[e * 2 + 1]);
+#pragma unroll
+          for (int b = 0; b < kBlocks; b++) {
+            const uint32_t v[4] = {kw[b].x, kw[b].y, kw[b].z, kw[b].w};
+            if (BF16)
+              Operand<BF16>::mul(c[b][s % kChains], qv, v[e] << 16, v[e] & 0xffff0000u);
+            else
+              Operand<BF16>::mul(c[b][s % kChains], qv, v[e * 2], v[e * 2 + 1]);
+          }
         }
       }
 #pragma unroll
-      for (int e = 0; e < 2; e++) {
-        float sum = 0.0f;
+      for (int b = 0; b < kBlocks; b++) {
 #pragma unroll
-        for (int ch = 0; ch < kChains; ch++) sum += c[ch][e] + c[ch][e + 2];
-        x[b][e] = key0 + b * 8 + 2 * t + e < end ? sum : -INFINITY;
-      }
-      if (score && g < heads) {
+        for (int e = 0; e < 2; e++) {
+          float sum = 0.0f;
+#pragma unroll
+          for (int ch = 0; ch < kChains; ch++) sum += c[b][ch][e] + c[b][ch][e + 2];
+          x[b][e] = sum;
+        }
         const int s = key0 + b * 8 + 2 * t;
-        if (s < end) score[s] = x[b][0];
-        if (s + 1 < end) score[s + 1] = x[b][1];
+        if (key0 + kKeys > end) {
+          if (s >= end) x[b][0] = -INFINITY;
+          if (s + 1 >= end) x[b][1] = -INFINITY;
+        }
+        if (score) {
+          if (s < end) score[s] = x[b][0];
+          if (s + 1 < end) score[s + 1] = x[b][1];
+        }
       }
-    }
-    float top = x[0][0];
+      float top = x[0][0];
 #pragma unroll
-    for (int b = 0; b < kBlocks; b++) top = fmaxf(top, fmaxf(x[b][0], x[b][1]));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // m moves only when a score passes it by kLazy (the first tile: from -inf).
-    if (__any_sync(0xffffffffu, top > m + kLazy)) {
-      const float to = top > m + kLazy ? top : m;
-      const float keep = to == m ? 1.0f : exp2f(m - to);
-      m = to, l *= keep;
+      for (int b = 0; b < kBlocks; b++) top = fmaxf(top, fmaxf(x[b][0], x[b][1]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // m moves only when a score passes it by kLazy (the first tile: from -inf).
+      if (__any_sync(0xffffffffu, top > m + kLazy)) {
+        const float to = top > m + kLazy ? top : m;
+        const float keep = to == m ? 1.0f : exp2_of(m - to);
+        m = to, l *= keep;
 #pragma unroll
-      for (int s = 0; s < kSteps; s++)
+        for (int s = 0; s < kSteps; s++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[s][e] *= keep;
-    }
+          for (int e = 0; e < 4; e++) o[s][e] *= keep;
+      }
 #pragma unroll
-    for (int b = 0; b < kBlocks; b++) {
-      const float p0 = exp2f(x[b][0] - m), p1 = exp2f(x[b][1] - m);
-      l += p0 + p1;
-      uint32_t p[4];
-      split(p0, p[0], p[1]);
-      split(p1, p[2], p[3]);
-      const uint32_t row = vt + (b * 8 + 2 * t) * S::kRow + ((g ^ (2 * t)) << 4);
+      for (int b = 0; b < kBlocks; b++) {
+        const float p0 = exp2_of(x[b][0] - m), p1 = exp2_of(x[b][1] - m);
+        l += p0 + p1;
+        uint32_t p[4];
+        split(p0, p[0], p[1]);
+        split(p1, p[2], p[3]);
+        const uint32_t vrow = vt + (b * 8 + 2 * t) * S::kRow + ((g ^ (2 * t)) << 4);
 #pragma unroll
-      for (int i = 0; i < S::kRow / 128; i++) {
-        const uint4 w0 = lds16(row + i * 128), w1 = lds16(row + S::kRow + i * 128);
-        const uint32_t v0[4] = {w0.x, w0.y, w0.z, w0.w}, v1[4] = {w1.x, w1.y, w1.z, w1.w};
+        for (int i = 0; i < S::kRow / 128; i++) {
+          const uint4 w0 = lds16(vrow + i * 128), w1 = lds16(vrow + S::kRow + i * 128);
+          const uint32_t v0[4] = {w0.x, w0.y, w0.z, w0.w}, v1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          if (BF16) {
-            Operand<BF16>::mul(o[i * 8 + e * 2], p, v0[e] << 16, v1[e] << 16);
-            Operand<BF16>::mul(o[i * 8 + e * 2 + 1], p, v0[e] & 0xffff0000u, v1[e] & 0xffff0000u);
-          } else {
-            Operand<BF16>::mul(o[i * 4 + e], p, v0[e], v1[e]);
+          for (int e = 0; e < 4; e++) {
+            if (BF16) {
+              Operand<BF16>::mul(o[i * 8 + e * 2], p, v0[e] << 16, v1[e] << 16);
+              Operand<BF16>::mul(o[i * 8 + e * 2 + 1], p, v0[e] & 0xffff0000u, v1[e] & 0xffff0000u);
+            } else {
+              Operand<BF16>::mul(o[i * 4 + e], p, v0[e], v1[e]);
+            }
           }
         }
       }
     }
-  }
-  copies_wait<0>();
-  l += __shfl_xor_sync(0xffffffffu, l, 1);
-  l += __shfl_xor_sync(0xffffffffu, l, 2);
-  __syncthreads();  // the buffers are free
+    __syncwarp();  // all lanes are done with the buffers
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
 
-  // Join the warps: sums through shared memory, [warp][head][DH].
-  float* sums = reinterpret_cast<float*>(smem);
+    // The sums of a pair done by this warp alone, of a piece of it, or (a whole
+    // pair of a CTA) of this warp's blocks, to be joined in shared memory.  A
+    // warp cuts at most two pairs, the one it continues and the one it begins.
+    const bool mine_all = !wk.whole && b1 - b0 == n_blocks;
+    const size_t slot = 2 * (size_t)w + (b0 == 0);
+    const float r = mine_all ? 1.0f / l : 1.0f;
+    float* y = a.y + ((size_t)at.seq * a.heads + head0) * a.dh;
+    float* stat = sc.stat ? sc.stat + 2 * ((size_t)at.seq * a.heads + head0) : nullptr;
+    float* sums = reinterpret_cast<float*>(smem + warp * S::kWarp);
+    float* to = wk.whole ? sums + g * kSum : (mine_all ? y : sc.part + slot * kHeads * a.dh) + g * a.dh;
+    if (g < heads) {
+      constexpr int kWide = BF16 ? 8 : 4;  // columns of a 16-byte piece: lane t holds 2 · kWide in a row
 #pragma unroll
-  for (int s = 0; s < kSteps; s++) {
-    constexpr int kWide = BF16 ? 8 : 4;  // columns of a 16-byte piece
-    const int d = s / kWide * (kWide * 8) + 2 * t * kWide + s % kWide;
-    float* to = sums + (warp * kHeads + g) * DH + d;
-    to[0] = o[s][0] + o[s][2];
-    to[kWide] = o[s][1] + o[s][3];
-  }
-  if (t == 0) s_m[warp][g] = m, s_l[warp][g] = l;
-  __syncthreads();
-  const bool cut = at.chunks > 1;
-  float* part = sc.part + (size_t)blockIdx.x * kHeads * a.dh;
-  float* part_ml = sc.part_ml + (size_t)blockIdx.x * kHeads * 2;
-  float* y = a.y + ((size_t)at.seq * a.heads + head0) * a.dh;
-  for (int e = threadIdx.x; e < heads * a.dh; e += kThreads) {
-    const int h = e / a.dh, d = e % a.dh;
-    float M = s_m[0][h], L = 0.0f, v = 0.0f;
+      for (int i = 0; i < kSteps / kWide; i++)
 #pragma unroll
-    for (int w = 1; w < kWarps; w++) M = fmaxf(M, s_m[w][h]);
+        for (int e = 0; e < 2; e++)
 #pragma unroll
-    for (int w = 0; w < kWarps; w++) {
-      const float f = s_l[w][h] > 0.0f ? exp2f(s_m[w][h] - M) : s_l[w][h];  // a warp without tiles: 0 (NaN stays)
-      L += s_l[w][h] * f;
-      v += sums[(w * kHeads + h) * DH + d] * f;
-    }
-    if (!cut) {
-      y[e] = v / L;
-      if (sc.stat && d == 0) {
-        float* st = sc.stat + 2 * ((size_t)at.seq * a.heads + head0 + h);
-        st[0] = M, st[1] = 1.0f / L;
-      }
-    } else {
-      part[e] = v;
-      if (d == 0) part_ml[2 * h] = M, part_ml[2 * h + 1] = L;
-    }
-  }
-  if (!cut) return;
-
-  // The last chunk of the (sequence, tile) to arrive joins all of them.
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    unsigned* cnt = sc.cnt + (size_t)at.seq * tiles + tile;
-    s_last = atomicAdd(cnt, 1u) == (unsigned)at.chunks - 1;
-    if (s_last) *cnt = 0;
-  }
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  const size_t cta0 = (size_t)blockIdx.x - (size_t)at.chunk * tiles;
-  const float* ml = sc.part_ml + cta0 * kHeads * 2;
-  const size_t ml_step = (size_t)tiles * kHeads * 2;
-  float* factor = reinterpret_cast<float*>(smem);  // [chunk][head]
-  for (int h = warp; h < heads; h += kWarps) {
-    float M = -INFINITY, L = 0.0f;
-    for (int c = lane; c < at.chunks; c += 32) M = fmaxf(M, __ldcg(ml + c * ml_step + 2 * h));
-    M = warp_max(M);
-    for (int c = lane; c < at.chunks; c += 32) {
-      const float f = exp2f(__ldcg(ml + c * ml_step + 2 * h) - M);
-      factor[c * kHeads + h] = f;
-      L += f * __ldcg(ml + c * ml_step + 2 * h + 1);
-    }
-    L = warp_sum(L);
-    if (lane == 0) {
-      s_m[0][h] = M, s_l[0][h] = 1.0f / L;
-      if (sc.stat) {
-        float* st = sc.stat + 2 * ((size_t)at.seq * a.heads + head0 + h);
-        st[0] = M, st[1] = 1.0f / L;
+          for (int c = 0; c < kWide; c += 4) {
+            const int d = i * (kWide * 8) + (2 * t + e) * kWide + c;
+            float v[4];
+#pragma unroll
+            for (int f = 0; f < 4; f++) v[f] = (o[i * kWide + c + f][e] + o[i * kWide + c + f][e + 2]) * r;
+            if (d < a.dh) *reinterpret_cast<float4*>(to + d) = make_float4(v[0], v[1], v[2], v[3]);
+          }
+      if (t == 0) {
+        if (wk.whole) {
+          s_m[warp][g] = m, s_l[warp][g] = l;
+        } else if (!mine_all) {
+          float* ml = sc.part_ml + (slot * kHeads + g) * 2;
+          ml[0] = m, ml[1] = l;
+        } else if (stat) {
+          stat[2 * g] = m, stat[2 * g + 1] = r;
+        }
       }
     }
-  }
-  __syncthreads();
-  const float* parts = sc.part + cta0 * kHeads * a.dh;
-  const size_t step = (size_t)tiles * kHeads * a.dh;
-  for (int e = threadIdx.x * 4; e < heads * a.dh; e += kThreads * 4) {
-    const int h = e / a.dh;  // dh is a multiple of 8
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-    for (int c = 0; c < at.chunks; c++) {
-      const float4 w = __ldcg(reinterpret_cast<const float4*>(parts + c * step + e));
-      const float f = factor[c * kHeads + h];
-      v.x = fmaf(w.x, f, v.x), v.y = fmaf(w.y, f, v.y), v.z = fmaf(w.z, f, v.z), v.w = fmaf(w.w, f, v.w);
+    if (wk.whole) {
+      __syncthreads();
+      for (int h = warp; h < heads; h += kWarps) {
+        float M = s_m[0][h], L = 0.0f, f[kWarps];  // warp 0 has a block: M > -inf unless the scores are not finite
+#pragma unroll
+        for (int x = 1; x < kWarps; x++) M = fmaxf(M, s_m[x][h]);
+#pragma unroll
+        for (int x = 0; x < kWarps; x++) {
+          f[x] = s_l[x][h] == 0.0f ? 0.0f : exp2_of(s_m[x][h] - M);  // 0: a warp without blocks
+          L += s_l[x][h] * f[x];
+        }
+        for (int d = lane; d < a.dh; d += 32) {
+          float v = 0.0f;
+#pragma unroll
+          for (int x = 0; x < kWarps; x++) v += reinterpret_cast<float*>(smem + x * S::kWarp)[h * kSum + d] * f[x];
+          y[h * a.dh + d] = v / L;
+        }
+        if (stat && lane == 0) stat[2 * h] = M, stat[2 * h + 1] = 1.0f / L;
+      }
+      __syncthreads();  // before the next pair's copies
     }
-    const float r = s_l[0][h];
-    y[e] = v.x * r, y[e + 1] = v.y * r, y[e + 2] = v.z * r, y[e + 3] = v.w * r;
+    }
+    // On to the next pair or the next sequence with tokens.
+    while (left && at.unit >= wk.tiles * wk.units_of(at.visible)) {
+      at.unit = 0, at.slots += (at.visible + 3) & ~3;
+      at.visible = visible_of(len_of(a.t, lens, ++at.seq), a.reach);
+    }
   }
+}
+
+// Four floats through L2, or zeros and no read; no branch, so that several are
+// on their way at once.
+__device__ __forceinline__ float4 load_if(const float* p, bool ok) {
+  float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %5, 0;\n @p ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];\n}\n"
+               : "+f"(r.x), "+f"(r.y), "+f"(r.z), "+f"(r.w)
+               : "l"(p), "r"((int)ok));
+  return r;
+}
+
+// Joins the pieces of cut pairs, a CTA per head of one.  Where there are fewer
+// pairs than warps, blockIdx.x counts them; else it counts the warps, and the
+// first warp of a cut pair joins it.
+constexpr int kJoin = 256, kMaxWarps = 148 * 4 * kWarps;
+__global__ void __launch_bounds__(kJoin)
+    k_paged_join(const __grid_constant__ PagedAttendArgs a, const __grid_constant__ Scratch sc,
+                 const __grid_constant__ Lens lens, const __grid_constant__ Work wk, bool by_pair) {
+  __shared__ float s_factor[kMaxWarps], s_red[2][kJoin / 32], s_sum[kJoin * 4];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int group = a.heads / a.key_heads, per_key = (group + kHeads - 1) / kHeads;
+  dependents_launch();
+  int seq, tile;
+  uint32_t origin, n;  // the pair's first unit, and its blocks
+  if (by_pair) {
+    seq = blockIdx.x / wk.tiles, tile = blockIdx.x % wk.tiles;
+    uint32_t before = 0;
+    for (int i = lane; i < seq; i += 32) before += wk.units_of(visible_of(len_of(a.t, lens, i), a.reach));
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) before += __shfl_xor_sync(0xffffffffu, before, x);
+    const uint32_t visible = visible_of(len_of(a.t, lens, seq), a.reach);
+    n = wk.blocks_of(visible);
+    origin = before * wk.tiles + tile * wk.units_of(visible);
+  } else {
+    // The pair that holds the last unit of warp blockIdx.x.
+    const uint32_t at = wk.first_unit(blockIdx.x + 1) - 1;
+    const Place p = locate(a.t, lens, a.reach, wk, at);
+    n = wk.blocks_of(p.visible);
+    seq = p.seq, tile = p.unit / wk.units_of(p.visible);
+    origin = at - (p.unit - tile * wk.units_of(p.visible));
+  }
+  dependency_wait();  // every CTA: that this kernel is done says that the one before it is
+  const uint32_t w0 = wk.taker_of(origin + wk.extra), w1 = n ? wk.taker_of(origin + wk.extra + n - 1) : w0;
+  const int kh = tile / per_key, head = tile % per_key * kHeads + blockIdx.y;  // of the key head's
+  if (n == 0 || w0 == w1 || (!by_pair && w0 != blockIdx.x) || head >= group) return;
+  const int parts = w1 - w0 + 1;
+  // Piece c: the first warp's second slot, then the others' first ones.
+  auto slot_of = [&](int c) { return (2 * (size_t)(w0 + c) + (c == 0)) * kHeads + blockIdx.y; };
+
+  // Threads of a group take 4 columns each, groups every so-manieth piece; the
+  // first pieces are on their way while the factors are worked out.
+  constexpr int kAtOnce = 8;
+  const int cols = a.dh / 4, groups = kJoin / cols, mine = min(tid / cols, groups - 1), d = tid % cols * 4;
+  float4 x[kAtOnce], v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto fetch = [&](int c) {
+#pragma unroll
+    for (int u = 0; u < kAtOnce; u++) x[u] = load_if(sc.part + slot_of(c + u * groups) * a.dh + d, c + u * groups < parts);
+  };
+  fetch(mine);
+
+  // M and l of the pieces, and each piece's factor.
+  float M = -INFINITY, L = 0.0f;
+  for (int c = tid; c < parts; c += kJoin) {
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(sc.part_ml) + slot_of(c));
+    s_factor[c] = ml.x;
+    const float to = fmaxf(M, ml.x);
+    L = (M == -INFINITY ? 0.0f : L * exp2_of(M - to)) + ml.y * exp2_of(ml.x - to);
+    M = to;
+  }
+  const float top = warp_max(M);
+  L = warp_sum(M == -INFINITY ? 0.0f : L * exp2_of(M - top));
+  if (lane == 0) s_red[0][warp] = top, s_red[1][warp] = L;
+  __syncthreads();
+  M = s_red[0][0], L = 0.0f;
+#pragma unroll
+  for (int w = 1; w < kJoin / 32; w++) M = fmaxf(M, s_red[0][w]);
+#pragma unroll
+  for (int w = 0; w < kJoin / 32; w++) L += s_red[0][w] == -INFINITY ? 0.0f : s_red[1][w] * exp2_of(s_red[0][w] - M);
+  for (int c = mine;;) {
+#pragma unroll
+    for (int u = 0; u < kAtOnce; u++) {
+      const int p = c + u * groups;
+      const float f = p < parts ? exp2_of(s_factor[min(p, parts - 1)] - M) : 0.0f;
+      v.x = fmaf(x[u].x, f, v.x), v.y = fmaf(x[u].y, f, v.y), v.z = fmaf(x[u].z, f, v.z), v.w = fmaf(x[u].w, f, v.w);
+    }
+    c += groups * kAtOnce;
+    if (c >= parts) break;
+    fetch(c);
+  }
+  if (tid < groups * cols) *reinterpret_cast<float4*>(&s_sum[mine * a.dh + d]) = v;
+  __syncthreads();
+  const size_t row = (size_t)seq * a.heads + kh * group + head;
+  for (int e = tid; e < a.dh; e += kJoin) {
+    float sum = 0.0f;
+    for (int w = 0; w < groups; w++) sum += s_sum[w * a.dh + e];
+    a.y[row * a.dh + e] = sum / L;
+  }
+  if (sc.stat && tid == 0) sc.stat[2 * row] = M, sc.stat[2 * row + 1] = 1.0f / L;
 }
 
 // weight[s] += Σ_h p_s over the key head's query heads, from the kept scores:
 // a thread per slot.
-__global__ void __launch_bounds__(kThreads) k_paged_weights(PagedAttendArgs a, Scratch sc) {
+__global__ void __launch_bounds__(kWeightKeys)
+    k_paged_weights(const __grid_constant__ PagedAttendArgs a, const __grid_constant__ Scratch sc,
+                    const __grid_constant__ Lens lens) {
   const int kh = blockIdx.x % a.key_heads, group = a.heads / a.key_heads;
-  const Place at = find_place(a.t, a.reach, kWeightKeys, blockIdx.x / a.key_heads);
-  const int lo = (int)a.t.lens[at.seq] - at.visible, padded = (at.visible + 3) & ~3;
-  const float* score = sc.score + at.before * a.heads + (size_t)kh * group * padded;
+  const Place at = locate(a.t, lens, a.reach, Work{kWeightKeys, 0, 0, 0, 1, false}, blockIdx.x / a.key_heads);
+  const int v = at.unit * kWeightKeys + threadIdx.x, padded = (at.visible + 3) & ~3;
+  if (v >= at.visible) return;
+  const uint32_t s = len_of(a.t, lens, at.seq) - at.visible + v, page = a.t.page_of(s);
+  float* w = a.weights + ((size_t)a.t.ids[(size_t)at.seq * a.t.per + page] * a.key_heads + kh) * a.t.page +
+             (s - page * a.t.page);
+  const float was = *w;
+  dependency_wait();
+  const float* score = sc.score + at.slots * a.heads + (size_t)kh * group * padded + v;
   const float* stat = sc.stat + 2 * ((size_t)at.seq * a.heads + kh * group);
-  for (int j = threadIdx.x; j < kWeightKeys; j += kThreads) {
-    const int v = at.chunk * kWeightKeys + j;
-    if (v >= at.visible) break;
-    float sum = 0.0f;
-    for (int h = 0; h < group; h++) sum += exp2f(score[(size_t)h * padded + v] - stat[2 * h]) * stat[2 * h + 1];
-    const int s = lo + v, page = s / a.t.page;
-    a.weights[((size_t)a.t.ids[(size_t)at.seq * a.t.per + page] * a.key_heads + kh) * a.t.page + s - page * a.t.page] +=
-        sum;
-  }
+  float sum = 0.0f;
+#pragma unroll 4
+  for (int h = 0; h < group; h++) sum += exp2_of(score[(size_t)h * padded] - stat[2 * h]) * stat[2 * h + 1];
+  *w = was + sum;
 }
 
-// y rows of idle sequences (their key heads have no CTA).
-__global__ void k_paged_idle(PagedAttendArgs a) {
-  const int i = blockIdx.x;
-  if (a.t.lens[i] != 0) return;
-  for (int e = threadIdx.x; e < a.heads * a.dh; e += blockDim.x) a.y[(size_t)i * a.heads * a.dh + e] = 0.0f;
-}
-
-// What a launch is cut into.
 struct Plan {
-  int keys, tiles, ctas;   // slots of a chunk; head tiles; CTAs in all
-  int weight_ctas;
-  bool cut, idle;
-  size_t slots;            // visible slots, each sequence's rounded up to 4
+  Work work;
+  uint32_t weight_ctas;
+  int pairs;
+  bool idle, cut;
+  size_t slots;  // visible slots, each sequence's rounded up to 4
 };
 
 int padded_dh(int dh) { return dh <= 64 ? 64 : dh <= 128 ? 128 : 256; }
 
+// Beginning and ending a pair takes a warp about as long as two blocks (4200
+// cycles against 1900 to 2400 a block): counted so, 16 ragged sequences of 8
+// key heads take 50 us, against 52 at one and 64 without.
+constexpr uint32_t kExtra = 2;
+// Pairs of up to this many blocks stay whole, a CTA each, joined in shared
+// memory: cut, a call of 97 slots takes 8.2 us instead of 7.7.
+constexpr uint32_t kWholeBlocks = 16;
+
 Plan plan_of(const PagedAttendArgs& a) {
   Plan p{};
-  const int group = a.heads / a.key_heads, size = a.bf16 ? 2 : 4, dh = padded_dh(a.dh);
-  p.tiles = a.key_heads * ((group + kHeads - 1) / kHeads);
-  const int row = dh * size, tile_keys = std::max(8, 4096 / row) * kWarps;
-  const int room = 148 * (!a.bf16 && dh == 256 ? 1 : 2);
-  long long total = 0, longest = 0, weight_ctas = 0;
+  const int group = a.heads / a.key_heads, dh = padded_dh(a.dh);
+  const int* cfg = kCfg[(a.bf16 ? 3 : 0) + (dh == 64 ? 0 : dh == 128 ? 1 : 2)];
+  Work& wk = p.work;
+  wk.keys = cfg[0], wk.tiles = a.key_heads * ((group + kHeads - 1) / kHeads);
+  p.pairs = a.t.n * wk.tiles;
+  uint32_t longest = 0, busy = 0;
   for (int i = 0; i < a.t.n; i++) {
-    const int v = visible_of(a.host_lens[i], a.reach);
-    total += v, longest = std::max<long long>(longest, v);
-    p.slots += (v + 3) & ~3;
-    p.idle |= v == 0;
-    weight_ctas += (long long)cdiv(v, kWeightKeys) * a.key_heads;
+    const uint32_t v = visible_of(a.host_lens[i], a.reach);
+    longest = std::max(longest, v), busy += v > 0;
+    p.slots += (v + 3) & ~3u;
   }
-  // Chunks of about 256 KB when there is work for many of them, else one for
-  // every place a CTA has on the GPU; at least one tile a warp.
-  long long keys = std::min<long long>((total * p.tiles + room - 1) / room, std::max(1, 262144 / (2 * row)));
-  keys = std::max(keys, (longest + kMaxChunks - 1) / kMaxChunks);
-  keys = std::max<long long>(1, (keys + tile_keys - 1) / tile_keys) * tile_keys;
-  p.keys = (int)keys;  // below 2^21: a sequence holds less than 2^30 slots
-  long long chunks = 0;
+  p.idle = busy < (uint32_t)a.t.n;
+  wk.whole = wk.blocks_of(longest) <= kWholeBlocks;
+  wk.extra = wk.whole ? 0 : kExtra;
+  uint64_t units = 0, weight_ctas = 0;
   for (int i = 0; i < a.t.n; i++) {
-    const long long c = (visible_of(a.host_lens[i], a.reach) + (long long)p.keys - 1) / p.keys;
-    chunks += c;
-    p.cut |= c > 1;
+    const uint32_t v = visible_of(a.host_lens[i], a.reach);
+    units += (uint64_t)wk.units_of(v) * wk.tiles;
+    weight_ctas += (uint64_t)(v + kWeightKeys - 1) / kWeightKeys * a.key_heads;
   }
-  SLM_REQUIRE(std::max(chunks * p.tiles, weight_ctas) < (1ll << 31), "paged_attend: too much work for one call");
-  p.weight_ctas = (int)weight_ctas;
-  p.ctas = (int)(chunks * p.tiles);
+  SLM_REQUIRE(std::max(units, weight_ctas) < (1ull << 31), "paged_attend: too much work for one call");
+  wk.units = (uint32_t)units, p.weight_ctas = (uint32_t)weight_ctas;
+  // A taker for every place on the GPU.
+  wk.takers = (uint32_t)std::min<uint64_t>(148 * cfg[2] * (wk.whole ? 1 : kWarps), units);
+  p.cut = !wk.whole && wk.takers > 1;
   return p;
 }
 
@@ -520,18 +706,31 @@ size_t carve(const PagedAttendArgs& a, const Plan& p, float* base, Scratch* sc) 
     at += round4(n);
     return r;
   };
-  const size_t parts = p.cut ? (size_t)p.ctas : 0;
-  sc->part = take(parts * kHeads * a.dh);
-  sc->part_ml = take(parts * kHeads * 2);
+  const size_t warps = p.cut ? p.work.takers : 0;
+  sc->part = take(2 * warps * kHeads * a.dh);
+  sc->part_ml = take(2 * warps * kHeads * 2);
   sc->stat = a.weights ? take((size_t)a.t.n * a.heads * 2) : nullptr;
   sc->score = a.weights ? take(p.slots * a.heads) : nullptr;
-  sc->cnt = a.counters;
   return at + 4;
 }
 
+// Launches a kernel that begins while the one before it still runs.
+template <class... P, class... A>
+void launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, cudaStream_t st, A... args) {
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c{};
+  c.gridDim = grid, c.blockDim = dim3(threads), c.stream = st, c.attrs = &at, c.numAttrs = 1;
+  SLM_CUDA(cudaLaunchKernelEx(&c, kernel, P(args)...));
+}
+
 template <bool BF16, int DH>
-void launch(const PagedAttendArgs& a, const Scratch& sc, const Plan& p, cudaStream_t st) {
-  k_paged_attend<BF16, DH><<<p.ctas, kThreads, Shape<BF16 ? 2 : 4, DH>::kSmem, st>>>(a, sc, p.keys, p.tiles);
+void launch(const PagedAttendArgs& a, const Scratch& sc, const Lens& lens, const Plan& p, cudaStream_t st) {
+  const bool q16 = ((uintptr_t)a.q & 15) == 0 && a.ldq % 4 == 0;  // q in 16-byte loads
+  const unsigned ctas = p.work.whole ? p.work.takers : cdiv(p.work.takers, kWarps);
+  k_paged_attend<BF16, DH><<<std::max(1u, ctas), kThreads, Shape<BF16 ? 2 : 4, DH>::kSmem, st>>>(a, sc, lens, p.work,
+                                                                                                  p.idle, q16);
 }
 
 template <bool BF16, int DH>
@@ -556,30 +755,25 @@ size_t paged_attend_scratch(const PagedAttendArgs& a) {
   return carve(a, plan_of(a), nullptr, &sc);
 }
 
-size_t paged_attend_counters(const PagedAttendArgs& a) {
-  const int group = a.heads / a.key_heads;
-  return (size_t)a.t.n * a.key_heads * ((group + kHeads - 1) / kHeads);
-}
-
 void paged_attend(const PagedAttendArgs& a, cudaStream_t st) {
   const Plan p = plan_of(a);
   Scratch sc;
   carve(a, p, a.scratch, &sc);
-  if (p.idle) {
-    k_paged_idle<<<a.t.n, 256, 0, st>>>(a);
-    SLM_LAUNCHED("k_paged_idle");
-  }
-  if (!p.ctas) return;
+  Lens lens;
+  if (a.t.n <= kLens) std::copy(a.host_lens, a.host_lens + a.t.n, lens.v);
   const int dh = padded_dh(a.dh);
   if (a.bf16)
-    dh == 64 ? launch<true, 64>(a, sc, p, st) : dh == 128 ? launch<true, 128>(a, sc, p, st) : launch<true, 256>(a, sc, p, st);
+    (dh == 64 ? launch<true, 64> : dh == 128 ? launch<true, 128> : launch<true, 256>)(a, sc, lens, p, st);
   else
-    dh == 64 ? launch<false, 64>(a, sc, p, st) : dh == 128 ? launch<false, 128>(a, sc, p, st) : launch<false, 256>(a, sc, p, st);
+    (dh == 64 ? launch<false, 64> : dh == 128 ? launch<false, 128> : launch<false, 256>)(a, sc, lens, p, st);
   SLM_LAUNCHED("k_paged_attend");
-  if (a.weights) {
-    k_paged_weights<<<p.weight_ctas, kThreads, 0, st>>>(a, sc);
-    SLM_LAUNCHED("k_paged_weights");
+  if (p.cut) {
+    const bool by_pair = p.pairs < (int)p.work.takers;
+    launch_after(k_paged_join, dim3(by_pair ? p.pairs : p.work.takers, std::min(kHeads, a.heads / a.key_heads)), kJoin,
+                 st, a, sc, lens, p.work, by_pair);
   }
+  if (a.weights && p.weight_ctas)
+    launch_after(k_paged_weights, dim3(p.weight_ctas), kWeightKeys, st, a, sc, lens);
 }
 
 }  // namespace slm

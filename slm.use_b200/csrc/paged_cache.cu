@@ -13,8 +13,8 @@ namespace {
 
 // Pool row of slot s of sequence i, key head h.
 __device__ __forceinline__ size_t pool_row(const PagedTable& t, int i, int s, int h, int key_heads) {
-  const uint32_t id = t.ids[(size_t)i * t.per + s / t.page];
-  return ((size_t)id * key_heads + h) * t.page + s % t.page;
+  const uint32_t page = t.page_of(s), id = t.ids[(size_t)i * t.per + page];
+  return ((size_t)id * key_heads + h) * t.page + (s - page * t.page);
 }
 
 struct Words {
