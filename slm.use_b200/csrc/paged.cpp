@@ -220,10 +220,14 @@ int slm_op_paged_evict(slm_ctx* c, slm_buf* kept, slm_buf* k, slm_buf* v, slm_bu
     Device dev(c);
     not_capturing(c, "paged_evict");
     ensure(kept, words);
-    for (size_t i = 0; i < from->host.seqs; i++) to->host.set_len(i, (uint32_t)std::min<size_t>(from->host.len(i), keep));
+    PagedEvictArgs a;
+    a.longest = 0;
+    for (size_t i = 0; i < from->host.seqs; i++) {
+      to->host.set_len(i, (uint32_t)std::min<size_t>(from->host.len(i), keep));
+      a.longest = std::max(a.longest, (int)from->host.len(i));
+    }
     flush(from);
     flush(to);
-    PagedEvictArgs a;
     a.from = on_device(from), a.to = on_device(to);
     a.key_heads = (int)p->key_heads, a.dh = (int)p->dh, a.bf16 = p->type == SLM_PAGES_BF16;
     a.keep = (int)keep, a.sinks = (int)sinks, a.recent = (int)recent;

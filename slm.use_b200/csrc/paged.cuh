@@ -5,7 +5,26 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "common.cuh"
+
 namespace slm {
+
+// A kernel may begin while the one before it in the stream still runs: what
+// follows `wait` sees all that the earlier one wrote.
+__device__ __forceinline__ void dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Launches a kernel that begins while the one before it still runs.
+template <class... P, class... A>
+inline void launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, cudaStream_t st, A... args) {
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c{};
+  c.gridDim = grid, c.blockDim = dim3(threads), c.stream = st, c.attrs = &at, c.numAttrs = 1;
+  SLM_CUDA(cudaLaunchKernelEx(&c, kernel, P(args)...));
+}
+
 
 // A table on the device and the pool's geometry.  Row s of sequence i, key
 // head h is row (ids[i·per + s / page] · key_heads + h) · page + s % page of
@@ -63,10 +82,12 @@ struct PagedEvictArgs {
   int key_heads, dh;
   bool bf16;
   int keep, sinks, recent;
+  int longest;  // the longest sequence's tokens
   void *k, *v;
   float* weights;
   uint32_t* kept;  // [n][key_heads][keep]
 };
+void paged_cache_prepare();  // as paged_prepare
 void paged_evict(const PagedEvictArgs& a, cudaStream_t st);
 
 // words[at[j]] = value[j] for j < n (≤ kPutWords): table updates, by value in

@@ -150,19 +150,19 @@ struct Operand<true> {
 // Pairs lie one after the other in units: `extra` (what beginning a pair costs,
 // in blocks) plus its blocks; with whole = true a pair is one unit, never cut.
 struct Work {
-  uint32_t keys, extra, units;  // units: in all
-  uint32_t takers;              // warps (CTAs if whole) that share them
+  uint32_t keys, extra;
+  uint32_t takers;              // warps (CTAs if whole) that share the units:
+  uint32_t each, more;          // `each` and one more for the first `more`
   int tiles;                    // pairs of a sequence
   bool whole;
   __host__ __device__ uint32_t blocks_of(uint32_t visible) const { return (visible + keys - 1) / keys; }
   __host__ __device__ uint32_t units_of(uint32_t visible) const {  // of a pair
     return visible == 0 ? 0 : whole ? 1 : blocks_of(visible) + extra;
   }
-  // Units are shared evenly: taker w has those from first_unit(w) on; taker_of
-  // is its inverse.
-  __device__ uint32_t first_unit(uint32_t w) const { return (uint32_t)((uint64_t)w * units / takers); }
+  __device__ uint32_t first_unit(uint32_t w) const { return w * each + min(w, more); }
   __device__ uint32_t taker_of(uint32_t unit) const {
-    return (uint32_t)((((uint64_t)unit + 1) * takers - 1) / units);
+    const uint32_t longer = more * (each + 1);
+    return unit < longer ? unit / (each + 1) : more + (unit - longer) / each;
   }
 };
 
@@ -202,11 +202,6 @@ __device__ __forceinline__ Place locate(const PagedTable& t, const Lens& lens, l
     p.unit -= n, p.slots += (p.visible + 3) & ~3;
   }
 }
-
-// A kernel may begin while the one before it in the stream still runs: what
-// follows `wait` sees all that the earlier one wrote.
-__device__ __forceinline__ void dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 template <bool BF16, int DH>
 __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
@@ -540,7 +535,8 @@ __device__ __forceinline__ float4 load_if(const float* p, bool ok) {
 // Joins the pieces of cut pairs, a CTA per head of one.  Where there are fewer
 // pairs than warps, blockIdx.x counts them; else it counts the warps, and the
 // first warp of a cut pair joins it.
-constexpr int kJoin = 256, kMaxWarps = 148 * 4 * kWarps;
+constexpr int kMaxWarps = 148 * 2 * kWarps;
+template <int kJoin>
 __global__ void __launch_bounds__(kJoin)
     k_paged_join(const __grid_constant__ PagedAttendArgs a, const __grid_constant__ Scratch sc,
                  const __grid_constant__ Lens lens, const __grid_constant__ Work wk, bool by_pair) {
@@ -632,7 +628,7 @@ __global__ void __launch_bounds__(kWeightKeys)
     k_paged_weights(const __grid_constant__ PagedAttendArgs a, const __grid_constant__ Scratch sc,
                     const __grid_constant__ Lens lens) {
   const int kh = blockIdx.x % a.key_heads, group = a.heads / a.key_heads;
-  const Place at = locate(a.t, lens, a.reach, Work{kWeightKeys, 0, 0, 0, 1, false}, blockIdx.x / a.key_heads);
+  const Place at = locate(a.t, lens, a.reach, Work{kWeightKeys, 0, 0, 0, 0, 1, false}, blockIdx.x / a.key_heads);
   const int v = at.unit * kWeightKeys + threadIdx.x, padded = (at.visible + 3) & ~3;
   if (v >= at.visible) return;
   const uint32_t s = len_of(a.t, lens, at.seq) - at.visible + v, page = a.t.page_of(s);
@@ -689,9 +685,10 @@ Plan plan_of(const PagedAttendArgs& a) {
     weight_ctas += (uint64_t)(v + kWeightKeys - 1) / kWeightKeys * a.key_heads;
   }
   SLM_REQUIRE(std::max(units, weight_ctas) < (1ull << 31), "paged_attend: too much work for one call");
-  wk.units = (uint32_t)units, p.weight_ctas = (uint32_t)weight_ctas;
+  p.weight_ctas = (uint32_t)weight_ctas;
   // A taker for every place on the GPU.
   wk.takers = (uint32_t)std::min<uint64_t>(148 * cfg[2] * (wk.whole ? 1 : kWarps), units);
+  if (wk.takers) wk.each = (uint32_t)(units / wk.takers), wk.more = (uint32_t)(units % wk.takers);
   p.cut = !wk.whole && wk.takers > 1;
   return p;
 }
@@ -712,17 +709,6 @@ size_t carve(const PagedAttendArgs& a, const Plan& p, float* base, Scratch* sc) 
   sc->stat = a.weights ? take((size_t)a.t.n * a.heads * 2) : nullptr;
   sc->score = a.weights ? take(p.slots * a.heads) : nullptr;
   return at + 4;
-}
-
-// Launches a kernel that begins while the one before it still runs.
-template <class... P, class... A>
-void launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, cudaStream_t st, A... args) {
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t c{};
-  c.gridDim = grid, c.blockDim = dim3(threads), c.stream = st, c.attrs = &at, c.numAttrs = 1;
-  SLM_CUDA(cudaLaunchKernelEx(&c, kernel, P(args)...));
 }
 
 template <bool BF16, int DH>
@@ -769,8 +755,12 @@ void paged_attend(const PagedAttendArgs& a, cudaStream_t st) {
   SLM_LAUNCHED("k_paged_attend");
   if (p.cut) {
     const bool by_pair = p.pairs < (int)p.work.takers;
-    launch_after(k_paged_join, dim3(by_pair ? p.pairs : p.work.takers, std::min(kHeads, a.heads / a.key_heads)), kJoin,
-                 st, a, sc, lens, p.work, by_pair);
+    const dim3 grid(by_pair ? p.pairs : p.work.takers, std::min(kHeads, a.heads / a.key_heads));
+    // Few pieces a pair: small CTAs, since there are many.
+    if ((int)p.work.takers < 32 * p.pairs && a.dh <= 128)
+      launch_after(k_paged_join<64>, grid, 64, st, a, sc, lens, p.work, by_pair);
+    else
+      launch_after(k_paged_join<256>, grid, 256, st, a, sc, lens, p.work, by_pair);
   }
   if (a.weights && p.weight_ctas)
     launch_after(k_paged_weights, dim3(p.weight_ctas), kWeightKeys, st, a, sc, lens);

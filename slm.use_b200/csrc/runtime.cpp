@@ -184,6 +184,7 @@ int slm_ctx_new(int device, slm_ctx** out) {
       SLM_CUDA(cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking));
       linear_prepare();
       paged_prepare();
+      paged_cache_prepare();
       c->err = static_cast<int*>(dev_alloc(sizeof(int) * 4));
       SLM_CUDA(cudaMemsetAsync(c->err, 0, sizeof(int) * 4, c->stream));
       SLM_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&c->err_host), sizeof(int) * 4, cudaHostAllocDefault));
