@@ -243,8 +243,8 @@ int slm_op_paged_attend(slm_ctx* ctx, slm_buf* y, slm_buf* scores, const slm_buf
  * token, stay as they were.  kept[i][key head][j] (32-bit words, seqs ×
  * key_heads × keep, grown as needed) is the slot in `from` that slot j of `to`
  * came from, 0xFFFFFFFF past the last.  `to`'s lengths become min(length,
- * keep).  Fails when `to`'s pages do not hold them, are listed twice in `to`,
- * or are listed in `from`. */
+ * keep).  Fails when `to`'s pages do not hold them, when two sequences of `to`
+ * list one page, or when the tables have a page in common. */
 int slm_op_paged_evict(slm_ctx* ctx, slm_buf* kept, slm_buf* k, slm_buf* v, slm_buf* weights, slm_table* from,
                        slm_table* to, size_t keep, size_t sinks, size_t recent, const slm_paged* p);
 

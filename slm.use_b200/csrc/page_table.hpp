@@ -14,6 +14,9 @@
 
 namespace slm {
 
+inline void table_require(bool ok, const char* msg) {
+  if (!ok) throw std::invalid_argument(msg);
+}
 inline void table_require(bool ok, const std::string& msg) {
   if (!ok) throw std::invalid_argument(msg);
 }
@@ -40,6 +43,7 @@ class PageTable {
     words.assign(seqs + seqs * per, 0);
     held.assign(seqs, 0);
     uses.assign(pages, 0);
+    listed.assign((pages + 63) / 64, 0);
   }
 
   const size_t seqs, per, page, pages;
@@ -47,6 +51,7 @@ class PageTable {
   std::vector<uint32_t> words;
   std::vector<uint32_t> held;  // pages of each sequence
   std::vector<uint32_t> uses;  // sequences that list each page
+  std::vector<uint64_t> listed;  // a bit per page: listed by any
   size_t shared = 0;           // pages listed by more than one
   size_t lo = 0, hi = 0;       // words changed since settle()
 
@@ -65,8 +70,16 @@ class PageTable {
     table_require(std::adjacent_find(sorted.begin(), sorted.end()) == sorted.end(),
                   "table_assign: a page comes twice in one sequence");
     uint32_t* row = words.data() + seqs + seq * per;
-    for (size_t j = 0; j < held[seq]; j++) shared -= --uses[row[j]] == 1;
-    for (size_t j = 0; j < n; j++) shared += ++uses[list[j]] == 2;
+    for (size_t j = 0; j < held[seq]; j++) {
+      const uint32_t id = row[j], left = --uses[id];
+      shared -= left == 1;
+      if (left == 0) listed[id / 64] &= ~((uint64_t)1 << id % 64);
+    }
+    for (size_t j = 0; j < n; j++) {
+      const uint32_t id = list[j];
+      shared += ++uses[id] == 2;
+      listed[id / 64] |= (uint64_t)1 << id % 64;
+    }
     size_t same = 0;  // a sequence that grew keeps its first pages
     while (same < n && same < held[seq] && row[same] == list[same]) same++;
     std::copy(list + same, list + n, row + same);
@@ -78,9 +91,9 @@ class PageTable {
     table_require(lens, "table_set_lens: bad arguments");
     table_require(n == seqs, "table_set_lens: one length per sequence");
     for (size_t i = 0; i < n; i++)
-      table_require(lens[i] <= held[i] * page, "table_set_lens: sequence " + std::to_string(i) + " has " +
-                                                   std::to_string(held[i]) + " pages, too few for " +
-                                                   std::to_string(lens[i]) + " tokens");
+      if (lens[i] > held[i] * page)
+        table_require(false, "table_set_lens: sequence " + std::to_string(i) + " has " + std::to_string(held[i]) +
+                                 " pages, too few for " + std::to_string(lens[i]) + " tokens");
     for (size_t i = 0; i < n; i++) set_len(i, lens[i]);
   }
 
@@ -107,16 +120,12 @@ class PageTable {
                   "paged_evict: the tables are of different sequences or pools");
     table_require(keep > 0 && keep < ((size_t)1 << 31), "paged_evict: bad budget");
     table_require(sinks <= keep && recent <= keep - sinks, "paged_evict: sinks and recent exceed the budget");
-    for (size_t i = 0; i < seqs; i++) {
-      const size_t n = std::min<size_t>(len(i), keep);
-      table_require(n <= to.held[i] * to.page,
-                    "paged_evict: sequence " + std::to_string(i) + " has too few pages to go to");
-      for (size_t j = 0; j * page < n; j++) {
-        const uint32_t id = to.ids(i)[j];
-        table_require(to.uses[id] == 1, "paged_evict: a page to go to is listed by two sequences");
-        table_require(uses[id] == 0, "paged_evict: a page to go to is one that tokens come from");
-      }
-    }
+    for (size_t i = 0; i < seqs; i++)
+      if (std::min<size_t>(len(i), keep) > to.held[i] * to.page)
+        table_require(false, "paged_evict: sequence " + std::to_string(i) + " has too few pages to go to");
+    table_require(to.shared == 0, "paged_evict: a page to go to is listed by two sequences");
+    for (size_t w = 0; w < listed.size(); w++)
+      table_require((listed[w] & to.listed[w]) == 0, "paged_evict: the tables have a page in common");
   }
 
  private:

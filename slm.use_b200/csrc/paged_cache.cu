@@ -88,27 +88,35 @@ __global__ void __launch_bounds__(kStoreThreads) k_paged_store(const __grid_cons
 }
 
 // ---------------------------------------------------------------------------
-// Evict, first part: which slots are kept.  A cluster of CTAs per pair (key
-// head, sequence), each CTA a contiguous slice of its slots with their weights
-// in shared memory, so memory is read once.  The lowest kept weight is found
-// digit by digit from the top (11, 11, 10 bits of an order-preserving integer):
-// every CTA counts its slice, the cluster's counts are added through
-// distributed shared memory, and the digit that holds the last kept weight is
-// the next prefix.  Latency bounds it (five cluster barriers).
+// Evict.  A cluster of CTAs per pair (key head, sequence), each CTA a
+// contiguous slice of its slots with their weights in shared memory, so memory
+// is read once.  The lowest kept weight is found digit by digit from the top
+// (11, 11, 10 bits of an order-preserving integer): every CTA counts its slice,
+// and one warp of each adds the cluster's counts through distributed shared
+// memory, first of 64 digits at a time, then of the 64 that hold the last kept
+// weight.  Latency bounds it.  A second kernel moves the kept tokens' rows,
+// bound by bytes (moved by the searching CTAs themselves, with too few loads in
+// flight, 16 ragged sequences of up to 32768 took 150 us instead of 98).
 // ---------------------------------------------------------------------------
-constexpr int kSelect = 1024, kDigits = 2048, kMaxCluster = 8;
+constexpr int kSelect = 512, kDigits = 2048, kGroup = 64, kMaxCluster = 8;
 constexpr int kSelectKeys = 40 * 1024;  // slots of a slice that shared memory holds; longer ones are read again
+constexpr int kSelectWarps = kSelect / 32;
 
-// Order of the weights as unsigned integers: NaN lowest, the two zeros equal.
+// Order of the weights as unsigned integers from 1 on: NaN lowest, the two
+// zeros equal.  0 stands for no slot, kHeld for one that does not compete.
+constexpr uint32_t kHeld = 0xffffffffu;
 __device__ __forceinline__ uint32_t order_of(float w) {
-  if (w != w) return 0;
+  if (w != w) return 1;
   const uint32_t b = __float_as_uint(w + 0.0f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  return (b & 0x80000000u ? ~b : b | 0x80000000u) + 1;
 }
 
-__global__ void __launch_bounds__(kSelect) k_paged_select(const __grid_constant__ PagedEvictArgs a, int room) {
+template <bool FITS>
+__global__ void __launch_bounds__(kSelect)
+    k_paged_select(const __grid_constant__ PagedEvictArgs a) {
   extern __shared__ uint32_t s_order[];
-  __shared__ int s_hist[3][kDigits], s_warp[32], s_digit, s_left, s_sure[33], s_tie[33];
+  __shared__ int s_hist[3][kDigits], s_coarse[3][kDigits / kGroup];
+  __shared__ int s_digit, s_left, s_sure[kSelectWarps + 1], s_tie[kSelectWarps + 1];
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = cluster.num_blocks(), part = cluster.block_rank();
   const int pair = blockIdx.x / parts, h = pair % a.key_heads, i = pair / a.key_heads;
@@ -118,133 +126,129 @@ __global__ void __launch_bounds__(kSelect) k_paged_select(const __grid_constant_
   dependents_launch();
   if (n <= a.keep) {  // all kept; uniform in the cluster
     for (int j = part * kSelect + t; j < a.keep; j += parts * kSelect) out[j] = j < n ? (uint32_t)j : 0xffffffffu;
-    return;
-  }
-  for (int d = t; d < 3 * kDigits; d += kSelect) (&s_hist[0][0])[d] = 0;
-  // A warp's slots lie together: 32 · rounds of them from first_slot on.
-  const int rounds = (n + parts * kSelect - 1) / (parts * kSelect);
-  const int slice = part * rounds * kSelect, mine = warp * rounds * 32;
-  const int lo = a.sinks, hi = n - a.recent;  // the slots that compete
-  auto order_at = [&](int j) -> uint32_t {    // j: in the slice
-    if (j < room) return s_order[j];
-    return order_of(a.weights[pool_row(a.from, i, slice + j, h, a.key_heads)]);
-  };
-  __syncthreads();
+  } else {
+    for (int d = t; d < 3 * kDigits; d += kSelect) (&s_hist[0][0])[d] = 0;
+    // A warp's slots lie together: 32 · rounds of them.
+    const int rounds = (n + parts * kSelect - 1) / (parts * kSelect);
+    const int slice = part * rounds * kSelect, mine = warp * rounds * 32 + lane;
+    const int lo = a.sinks, hi = n - a.recent;  // the slots that compete
+    auto fetch = [&](int j) -> uint32_t {       // j: in the slice
+      const int s = slice + j;
+      if (s >= n) return 0;
+      return s < lo || s >= hi ? kHeld : order_of(a.weights[pool_row(a.from, i, s, h, a.key_heads)]);
+    };
+    auto order_at = [&](int r) -> uint32_t {
+      const int j = mine + r * 32;
+      return FITS || j < kSelectKeys ? s_order[j] : fetch(j);
+    };
+    __syncthreads();
 #pragma unroll 4
-  for (int r = 0; r < rounds; r++) {
-    const int j = mine + r * 32 + lane, s = slice + j;
-    uint32_t o = 0;
-    if (s < n) o = order_of(a.weights[pool_row(a.from, i, s, h, a.key_heads)]);
-    if (j < room) s_order[j] = o;
-    if (s >= lo && s < hi) atomicAdd(&s_hist[0][o >> 21], 1);
-  }
-  uint32_t prefix = 0;
-  int need = a.keep - a.sinks - a.recent;  // how many of them are kept
+    for (int r = 0; r < rounds; r++) {
+      const uint32_t o = fetch(mine + r * 32);
+      if (FITS || mine + r * 32 < kSelectKeys) s_order[mine + r * 32] = o;
+      if (o != 0 && o != kHeld) atomicAdd(&s_hist[0][o >> 21], 1);
+    }
+    uint32_t prefix = 0;
+    int need = a.keep - a.sinks - a.recent;  // how many of those that compete are kept
+    if (need == 0) prefix = kHeld - 1;
 #pragma unroll
-  for (int pass = 0; pass < 3; pass++) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, digits = pass == 2 ? 1024 : 2048;
-    if (pass > 0) {
+    for (int pass = 0; pass < 3; pass++) {
+      if (need == 0) break;  // uniform in the cluster
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+      if (pass > 0) {
 #pragma unroll 4
-      for (int r = 0; r < rounds; r++) {
-        const int j = mine + r * 32 + lane, s = slice + j;
-        if (s < lo || s >= hi) continue;
-        const uint32_t o = order_at(j);
-        if (o >> (shift + (pass == 2 ? 10 : 11)) == prefix >> (shift + (pass == 2 ? 10 : 11)))
-          atomicAdd(&s_hist[pass][(o >> shift) & (digits - 1)], 1);
+        for (int r = 0; r < rounds; r++) {
+          const uint32_t o = order_at(r);
+          if (o >> (shift + bits) == prefix >> (shift + bits)) atomicAdd(&s_hist[pass][(o >> shift) & ((1 << bits) - 1)], 1);
+        }
       }
-    }
-    cluster.sync();
-    // Thread t: the cluster's counts of digits top - 2t and the one below, from the top.
-    const int d1 = kDigits - 1 - 2 * t, d0 = d1 - 1;
-    int c1 = 0, c0 = 0;
-    for (int p = 0; p < parts; p++) {
-      const int* from = cluster.map_shared_rank(s_hist[pass], p);
-      c1 += from[d1], c0 += from[d0];
-    }
-    int upto = c1 + c0;
+      __syncthreads();
+      // Counts of 64 digits at a time: coarse digit c of this CTA.
+      for (int c = warp; c < kDigits / kGroup; c += kSelectWarps) {
+        const int v = __reduce_add_sync(0xffffffffu, s_hist[pass][c * kGroup + lane] + s_hist[pass][c * kGroup + 32 + lane]);
+        if (lane == 0) s_coarse[pass][c] = v;
+      }
+      cluster.sync();
+      if (warp == 0) {
+        // From the top: the coarse digit that holds the need-th largest, then the digit.
+        int left = need, digit = 0;
 #pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, x);
-      if (lane >= x) upto += v;
+        for (int level = 0; level < 3; level++) {  // 32 coarse digits; then its upper and lower 32 digits
+          int c = 0;
+          const int at = level == 0 ? 31 - lane : digit * kGroup + (level == 1 ? 63 : 31) - lane;
+          if (level == 2 && s_left > 0) break;
+          for (int p = 0; p < parts; p++)
+            c += (level == 0 ? cluster.map_shared_rank(s_coarse[pass], p) : cluster.map_shared_rank(s_hist[pass], p))[at];
+          int upto = c;
+#pragma unroll
+          for (int x = 1; x < 32; x <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, x);
+            if (lane >= x) upto += v;
+          }
+          const unsigned reached = __ballot_sync(0xffffffffu, upto >= left);
+          if (level == 0) {
+            const int src = __ffs(reached) - 1;
+            left -= __shfl_sync(0xffffffffu, upto - c, src);
+            digit = 31 - src;
+            if (lane == 0) s_left = 0;
+            __syncwarp();
+          } else if (reached) {
+            const int src = __ffs(reached) - 1;
+            const int above = __shfl_sync(0xffffffffu, upto - c, src);
+            if (lane == src) s_digit = at, s_left = left - above;
+            __syncwarp();
+          } else {
+            left -= __shfl_sync(0xffffffffu, upto, 31);
+          }
+        }
+      }
+      __syncthreads();
+      prefix |= (uint32_t)s_digit << shift, need = s_left;
     }
-    if (lane == 31) s_warp[warp] = upto;
+    // Above `prefix`: kept; equal to it: the first `need`.  A kept slot's place
+    // is the number of sure ones before it and of ties before it, up to `need`.
+    int sure = 0, tie = 0;
+#pragma unroll 4
+    for (int r = 0; r < rounds; r++) {
+      const uint32_t o = order_at(r);
+      sure += __popc(__ballot_sync(0xffffffffu, o > prefix)), tie += __popc(__ballot_sync(0xffffffffu, o == prefix));
+    }
+    if (lane == 0) s_sure[warp] = sure, s_tie[warp] = tie;
     __syncthreads();
     if (warp == 0) {
-      int v = s_warp[lane];
+      int a0 = lane < kSelectWarps ? s_sure[lane] : 0, b0 = lane < kSelectWarps ? s_tie[lane] : 0;
+      const int a1 = a0, b1 = b0;
 #pragma unroll
       for (int x = 1; x < 32; x <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, v, x);
-        if (lane >= x) v += u;
+        const int u = __shfl_up_sync(0xffffffffu, a0, x), v = __shfl_up_sync(0xffffffffu, b0, x);
+        if (lane >= x) a0 += u, b0 += v;
       }
-      s_warp[lane] = v;
+      if (lane < kSelectWarps) s_sure[lane] = a0 - a1, s_tie[lane] = b0 - b1;
+      if (lane == 31) s_sure[kSelectWarps] = a0, s_tie[kSelectWarps] = b0;
     }
-    __syncthreads();
-    const int above = upto - (c1 + c0) + (warp ? s_warp[warp - 1] : 0);  // counts of higher digits
-    // The digit that holds the need-th largest (need 0: above all, the top digit's upper end).
-    if (above < need && above + c1 + c0 >= need) {
-      const bool first = above + c1 >= need;
-      s_digit = first ? d1 : d0;
-      s_left = need - above - (first ? 0 : c1);
+    cluster.sync();
+    sure = s_sure[warp], tie = s_tie[warp];
+    for (int p = 0; p < part; p++) {
+      sure += cluster.map_shared_rank(s_sure, p)[kSelectWarps];
+      tie += cluster.map_shared_rank(s_tie, p)[kSelectWarps];
     }
-    if (need == 0 && t == 0) s_digit = digits - 1, s_left = 0;
-    __syncthreads();
-    prefix |= (uint32_t)s_digit << shift, need = s_left;
-  }
-  // Above `prefix`: kept; equal to it: the first `need`.  A kept slot's place is
-  // the number of sure ones before it and of ties before it, up to `need`.
-  int sure = 0, tie = 0;
+    const unsigned below = (1u << lane) - 1;
 #pragma unroll 4
-  for (int r = 0; r < rounds; r++) {
-    const int j = mine + r * 32 + lane, s = slice + j;
-    bool is_sure = s < n && (s < lo || s >= hi), is_tie = false;
-    if (s >= lo && s < hi) {
-      const uint32_t o = order_at(j);
-      is_sure = o > prefix, is_tie = o == prefix;
+    for (int r = 0; r < rounds; r++) {
+      const uint32_t o = order_at(r);
+      const unsigned sures = __ballot_sync(0xffffffffu, o > prefix), ties = __ballot_sync(0xffffffffu, o == prefix);
+      const int tie_rank = tie + __popc(ties & below);
+      if (o > prefix || (o == prefix && tie_rank < need))
+        out[sure + __popc(sures & below) + min(tie_rank, need)] = (uint32_t)(slice + mine + r * 32);
+      sure += __popc(sures), tie += __popc(ties);
     }
-    sure += __popc(__ballot_sync(0xffffffffu, is_sure)), tie += __popc(__ballot_sync(0xffffffffu, is_tie));
-  }
-  if (lane == 0) s_sure[warp] = sure, s_tie[warp] = tie;
-  __syncthreads();
-  if (warp == 0) {
-    int a0 = s_sure[lane], b0 = s_tie[lane];
-    const int a1 = a0, b1 = b0;
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, a0, x), v = __shfl_up_sync(0xffffffffu, b0, x);
-      if (lane >= x) a0 += u, b0 += v;
-    }
-    s_sure[lane] = a0 - a1, s_tie[lane] = b0 - b1;
-    if (lane == 31) s_sure[32] = a0, s_tie[32] = b0;
-  }
-  cluster.sync();
-  sure = s_sure[warp], tie = s_tie[warp];
-  for (int p = 0; p < part; p++) {
-    sure += cluster.map_shared_rank(s_sure, p)[32];
-    tie += cluster.map_shared_rank(s_tie, p)[32];
-  }
-  const unsigned below = (1u << lane) - 1;
-  for (int r = 0; r < rounds; r++) {
-    const int j = mine + r * 32 + lane, s = slice + j;
-    bool is_sure = s < n && (s < lo || s >= hi), is_tie = false;
-    if (s >= lo && s < hi) {
-      const uint32_t o = order_at(j);
-      is_sure = o > prefix, is_tie = o == prefix;
-    }
-    const unsigned sures = __ballot_sync(0xffffffffu, is_sure), ties = __ballot_sync(0xffffffffu, is_tie);
-    const int tie_rank = tie + __popc(ties & below);
-    if (is_sure || (is_tie && tie_rank < need))
-      out[sure + __popc(sures & below) + min(tie_rank, need)] = (uint32_t)s;
-    sure += __popc(sures), tie += __popc(ties);
   }
   cluster.sync();  // no CTA leaves while others read its shared memory
 }
 
-// ---------------------------------------------------------------------------
-// Evict, second part: the kept tokens' K, V and weight rows.  Bytes bound it.
-// A CTA moves up to kMoveRows tokens of one pair in 16-byte pieces.
-// ---------------------------------------------------------------------------
+// Moves `rows` kept tokens of a pair: K, V and weight rows in 16-byte pieces
+// (`pieces` a row; e / pieces = e · by_pieces >> 32).
 constexpr int kMoveThreads = 256, kMoveRows = 64;
-
 __global__ void __launch_bounds__(kMoveThreads)
     k_paged_move(const __grid_constant__ PagedEvictArgs a, int pieces, uint32_t by_pieces, int rows) {
   __shared__ uint32_t s_from[kMoveRows], s_to[kMoveRows];
@@ -271,7 +275,7 @@ __global__ void __launch_bounds__(kMoveThreads)
 #pragma unroll
     for (int u = 0; u < kAtOnce; u++) {
       const uint32_t e = min(e0 + u * kMoveThreads, total - 1);
-      const uint32_t r = __umulhi(e, by_pieces), c = e - r * pieces;
+      const uint32_t r = pieces == 1 ? e : __umulhi(e, by_pieces), c = e - r * pieces;
       const size_t from = (size_t)s_from[r] * pieces + c;
       to[u] = (size_t)s_to[r] * pieces + c;
       kw[u] = ks[from], vw[u] = vs[from];
@@ -285,8 +289,9 @@ __global__ void __launch_bounds__(kMoveThreads)
 }  // namespace
 
 void paged_cache_prepare() {
-  SLM_CUDA(cudaFuncSetAttribute(k_paged_select, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                kSelectKeys * (int)sizeof(uint32_t)));
+  const int bytes = kSelectKeys * (int)sizeof(uint32_t);
+  for (auto k : {k_paged_select<false>, k_paged_select<true>})
+    SLM_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
 }
 
 void table_put(uint32_t* words, const uint32_t* at, const uint32_t* value, int n, cudaStream_t st) {
@@ -309,25 +314,27 @@ void paged_store(const PagedStoreArgs& a, cudaStream_t st) {
 }
 
 void paged_evict(const PagedEvictArgs& a, cudaStream_t st) {
-  // As many CTAs a pair as fill the GPU twice, with a slot at least a thread.
+  // As many CTAs a pair as fill the GPU, with two slots at least a thread.
+#ifndef PARTS
+#define PARTS 4
+#endif
   const size_t pairs = (size_t)a.from.n * a.key_heads;
   int parts = 1;
-  while (parts < kMaxCluster && pairs * parts * 2 <= 148 * 2 && a.longest > kSelect * parts) parts *= 2;
-  const int rounds = (a.longest + parts * kSelect - 1) / (parts * kSelect);
-  const int room = std::min(std::max(rounds, 1) * kSelect, kSelectKeys);
+  while (parts < kMaxCluster && pairs * parts * 2 <= 148 * PARTS && a.longest > 2 * kSelect * parts) parts *= 2;
+  const int rounds = std::max(1, (a.longest + parts * kSelect - 1) / (parts * kSelect));
+  const bool fits = rounds * kSelect <= kSelectKeys;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeClusterDimension;
   at.val.clusterDim.x = (unsigned)parts, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
   cudaLaunchConfig_t c{};
   c.gridDim = dim3((unsigned)(pairs * parts)), c.blockDim = dim3(kSelect), c.stream = st;
-  c.dynamicSmemBytes = room * sizeof(uint32_t), c.attrs = &at, c.numAttrs = 1;
-  SLM_CUDA(cudaLaunchKernelEx(&c, k_paged_select, a, room));
-  // 16-byte pieces of a row; e / pieces = e · by >> 32 for e < 64 · 64.
-  const int pieces = a.dh * (a.bf16 ? 2 : 4) / 16;
-  const uint32_t by = (uint32_t)((((uint64_t)1 << 32) + pieces - 1) / pieces);
-  const int rows = std::min(kMoveRows, std::max(8, 2048 / pieces));
+  c.dynamicSmemBytes = std::min(rounds * kSelect, kSelectKeys) * sizeof(uint32_t), c.attrs = &at, c.numAttrs = 1;
+  SLM_CUDA(cudaLaunchKernelEx(&c, fits ? k_paged_select<true> : k_paged_select<false>, a));
   const int most = std::min(a.keep, a.longest);
   if (most == 0) return;
+  // e / pieces = e · by >> 32 for e < 64 · 64 (one piece: not used).
+  const int pieces = a.dh * (a.bf16 ? 2 : 4) / 16, rows = std::min(kMoveRows, std::max(8, 2048 / pieces));
+  const uint32_t by = (uint32_t)((((uint64_t)1 << 32) + pieces - 1) / pieces);
   launch_after(k_paged_move, dim3(cdiv(most, rows), a.key_heads, a.from.n), kMoveThreads, st, a, pieces, by, rows);
 }
 

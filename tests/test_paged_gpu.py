@@ -360,6 +360,9 @@ EVICT = [
     ([9000, 20, 5000], 2, 32, 16, True, 4097, 4, 1000, "random"),
     ([70000], 2, 16, 64, True, 20001, 4, 100, "ties"),
     ([300], 1, 256, 7, False, 20, 1, 2, "tiny"),
+    ([(i * 97) % 1300 for i in range(40)], 3, 24, 16, True, 500, 2, 64, "random"),
+    ([(i * 97) % 1300 for i in range(40)], 4, 64, 8, False, 500, 0, 0, "ties"),
+    ([500000], 1, 8, 256, True, 70000, 4, 100, "random"),
 ]
 
 
