@@ -347,6 +347,7 @@ class Ops:
     def __init__(self, ctx: Context):
         self.ctx = ctx
         self._c = ctx._h
+        self._paged_key = None
 
     @staticmethod
     def _at(x):
@@ -448,34 +449,40 @@ class Ops:
     # [pages][key_heads][page][dh] values, f32 or, with bf16=True, bf16 values two to a float; weights
     # (optional but for paged_evict) is [pages][key_heads][page].
 
+    def _paged(self, *key):
+        """byref of the C struct of (heads, key_heads, dh, reach, scale, bf16); calls in a loop repeat the last one's."""
+        if key != self._paged_key:
+            *fields, bf16 = key
+            self._paged_c = _Paged(*fields, SLM_PAGES_BF16 if bf16 else SLM_PAGES_F32)
+            self._paged_key, self._paged_ref = key, _c.byref(self._paged_c)
+        return self._paged_ref
+
     def paged_store(self, k: Buf, v: Buf, table: Table, ksrc, vsrc, *, m: int, key_heads: int, dh: int,
                     first: int = 0, count: int | None = None, ldk: int | None = None, ldv: int | None = None,
                     bf16: bool = False, weights: Buf | None = None) -> None:
         """The last m tokens of sequences first .. first + count - 1 (count None: all that follow)."""
         (kb, ko), (vb, vo) = self._at(ksrc), self._at(vsrc)
         width = key_heads * dh
-        p = _Paged(0, key_heads, dh, 0, 0.0, SLM_PAGES_BF16 if bf16 else SLM_PAGES_F32)
-        _check(lib().slm_op_paged_store(self._c, k._h, v._h, weights._h if weights else None, table._h, first,
+        _check(lib().slm_op_paged_store(self._c, k._h, v._h, None if weights is None else weights._h, table._h, first,
                                         table.seqs - first if count is None else count, kb._h, ko,
                                         width if ldk is None else ldk, vb._h, vo, width if ldv is None else ldv, m,
-                                        _c.byref(p)))
+                                        self._paged(0, key_heads, dh, 0, 0.0, bf16)))
 
     def paged_attend(self, y: Buf, scores: Buf, q, k: Buf, v: Buf, table: Table, *, heads: int, key_heads: int,
                      dh: int, scale: float, reach: int | None = None, ldq: int | None = None, bf16: bool = False,
                      weights: Buf | None = None) -> None:
         """One query per sequence; reach None is unbounded; weights grow by what each token draws."""
         qb, qo = self._at(q)
-        p = _Paged(heads, key_heads, dh, SIZE_MAX if reach is None else reach, scale,
-                   SLM_PAGES_BF16 if bf16 else SLM_PAGES_F32)
         _check(lib().slm_op_paged_attend(self._c, y._h, scores._h, qb._h, qo, heads * dh if ldq is None else ldq, k._h,
-                                         v._h, weights._h if weights else None, table._h, _c.byref(p)))
+                                         v._h, None if weights is None else weights._h, table._h,
+                                         self._paged(heads, key_heads, dh, SIZE_MAX if reach is None else reach, scale,
+                                                     bf16)))
 
     def paged_evict(self, kept: Buf, k: Buf, v: Buf, weights: Buf, src: Table, dst: Table, *, keep: int, sinks: int,
                     recent: int, key_heads: int, dh: int, bf16: bool = False) -> None:
         """At most `keep` tokens per sequence and key head, from src's pages to dst's; kept holds 32-bit words."""
-        p = _Paged(0, key_heads, dh, 0, 0.0, SLM_PAGES_BF16 if bf16 else SLM_PAGES_F32)
         _check(lib().slm_op_paged_evict(self._c, kept._h, k._h, v._h, weights._h, src._h, dst._h, keep, sinks, recent,
-                                        _c.byref(p)))
+                                        self._paged(0, key_heads, dh, 0, 0.0, bf16)))
 
 
 def attend_noalloc(ctx: Context, y: Buf, q: Buf, k: Buf, v: Buf, *, pos: int, m: int, reach: int | None, gap: int,

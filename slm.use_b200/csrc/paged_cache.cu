@@ -111,11 +111,22 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return (b & 0x80000000u ? ~b : b | 0x80000000u) + 1;
 }
 
+// Inclusive sums over the lanes of a warp.
+__device__ __forceinline__ int scan_up(int v) {
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, x);
+    if ((threadIdx.x & 31) >= x) v += u;
+  }
+  return v;
+}
+
 template <bool FITS>
 __global__ void __launch_bounds__(kSelect)
     k_paged_select(const __grid_constant__ PagedEvictArgs a) {
   extern __shared__ uint32_t s_order[];
-  __shared__ int s_hist[3][kDigits], s_coarse[3][kDigits / kGroup];
+  __shared__ __align__(8) int s_hist[3][kDigits];
+  __shared__ int s_coarse[3][kDigits / kGroup];
   __shared__ int s_digit, s_left, s_sure[kSelectWarps + 1], s_tie[kSelectWarps + 1];
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = cluster.num_blocks(), part = cluster.block_rank();
@@ -142,11 +153,27 @@ __global__ void __launch_bounds__(kSelect)
       return FITS || j < kSelectKeys ? s_order[j] : fetch(j);
     };
     __syncthreads();
-#pragma unroll 4
-    for (int r = 0; r < rounds; r++) {
-      const uint32_t o = fetch(mine + r * 32);
-      if (FITS || mine + r * 32 < kSelectKeys) s_order[mine + r * 32] = o;
-      if (o != 0 && o != kHeld) atomicAdd(&s_hist[0][o >> 21], 1);
+    // Several slots' page ids, then weights, on their way at once.
+    constexpr int kAtOnce = 8;
+    const uint32_t* ids = a.from.ids + (size_t)i * a.from.per;
+    for (int r0 = 0; r0 < rounds; r0 += kAtOnce) {
+      uint32_t row[kAtOnce];
+      float w[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; u++) {
+        const uint32_t s = min(slice + mine + (r0 + u) * 32, n - 1), page = a.from.page_of(s);
+        row[u] = (ids[page] * a.key_heads + h) * a.from.page + (s - page * a.from.page);
+      }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; u++) w[u] = a.weights[row[u]];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; u++) {
+        const int j = mine + (r0 + u) * 32, s = slice + j;
+        if (r0 + u >= rounds) break;
+        const uint32_t o = s >= n ? 0 : s < lo || s >= hi ? kHeld : order_of(w[u]);
+        if (FITS || j < kSelectKeys) s_order[j] = o;
+        if (o != 0 && o != kHeld) atomicAdd(&s_hist[0][o >> 21], 1);
+      }
     }
     uint32_t prefix = 0;
     int need = a.keep - a.sinks - a.recent;  // how many of those that compete are kept
@@ -170,36 +197,29 @@ __global__ void __launch_bounds__(kSelect)
       }
       cluster.sync();
       if (warp == 0) {
-        // From the top: the coarse digit that holds the need-th largest, then the digit.
-        int left = need, digit = 0;
+        // From the top: the coarse digit that holds the need-th largest, then
+        // the digit, lane by lane two of them.
+        int c = 0;
 #pragma unroll
-        for (int level = 0; level < 3; level++) {  // 32 coarse digits; then its upper and lower 32 digits
-          int c = 0;
-          const int at = level == 0 ? 31 - lane : digit * kGroup + (level == 1 ? 63 : 31) - lane;
-          if (level == 2 && s_left > 0) break;
-          for (int p = 0; p < parts; p++)
-            c += (level == 0 ? cluster.map_shared_rank(s_coarse[pass], p) : cluster.map_shared_rank(s_hist[pass], p))[at];
-          int upto = c;
+        for (int p = 0; p < kMaxCluster; p++)
+          if (p < parts) c += cluster.map_shared_rank(s_coarse[pass], p)[31 - lane];
+        int upto = scan_up(c);
+        int src = __ffs(__ballot_sync(0xffffffffu, upto >= need)) - 1;
+        const int left = need - __shfl_sync(0xffffffffu, upto - c, src);
+        const int top = (31 - src) * kGroup + kGroup - 2 - 2 * lane;  // this lane's lower digit
+        int2 both = make_int2(0, 0);
 #pragma unroll
-          for (int x = 1; x < 32; x <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, x);
-            if (lane >= x) upto += v;
+        for (int p = 0; p < kMaxCluster; p++)
+          if (p < parts) {
+            const int2 v = *reinterpret_cast<const int2*>(cluster.map_shared_rank(s_hist[pass], p) + top);
+            both.x += v.x, both.y += v.y;
           }
-          const unsigned reached = __ballot_sync(0xffffffffu, upto >= left);
-          if (level == 0) {
-            const int src = __ffs(reached) - 1;
-            left -= __shfl_sync(0xffffffffu, upto - c, src);
-            digit = 31 - src;
-            if (lane == 0) s_left = 0;
-            __syncwarp();
-          } else if (reached) {
-            const int src = __ffs(reached) - 1;
-            const int above = __shfl_sync(0xffffffffu, upto - c, src);
-            if (lane == src) s_digit = at, s_left = left - above;
-            __syncwarp();
-          } else {
-            left -= __shfl_sync(0xffffffffu, upto, 31);
-          }
+        upto = scan_up(both.x + both.y);
+        src = __ffs(__ballot_sync(0xffffffffu, upto >= left)) - 1;
+        if (lane == src) {
+          const int rest = left - (upto - both.x - both.y);  // after the digits above this lane's
+          s_digit = both.y >= rest ? top + 1 : top;
+          s_left = both.y >= rest ? rest : rest - both.y;
         }
       }
       __syncthreads();
@@ -216,13 +236,8 @@ __global__ void __launch_bounds__(kSelect)
     if (lane == 0) s_sure[warp] = sure, s_tie[warp] = tie;
     __syncthreads();
     if (warp == 0) {
-      int a0 = lane < kSelectWarps ? s_sure[lane] : 0, b0 = lane < kSelectWarps ? s_tie[lane] : 0;
-      const int a1 = a0, b1 = b0;
-#pragma unroll
-      for (int x = 1; x < 32; x <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, a0, x), v = __shfl_up_sync(0xffffffffu, b0, x);
-        if (lane >= x) a0 += u, b0 += v;
-      }
+      const int a1 = lane < kSelectWarps ? s_sure[lane] : 0, b1 = lane < kSelectWarps ? s_tie[lane] : 0;
+      const int a0 = scan_up(a1), b0 = scan_up(b1);
       if (lane < kSelectWarps) s_sure[lane] = a0 - a1, s_tie[lane] = b0 - b1;
       if (lane == 31) s_sure[kSelectWarps] = a0, s_tie[kSelectWarps] = b0;
     }
@@ -314,13 +329,11 @@ void paged_store(const PagedStoreArgs& a, cudaStream_t st) {
 }
 
 void paged_evict(const PagedEvictArgs& a, cudaStream_t st) {
-  // As many CTAs a pair as fill the GPU, with two slots at least a thread.
-#ifndef PARTS
-#define PARTS 4
-#endif
+  // As many CTAs a pair as fill the GPU (four an SM; 93 us for 16 ragged
+  // sequences of up to 32768 against 98 with two), two slots at least a thread.
   const size_t pairs = (size_t)a.from.n * a.key_heads;
   int parts = 1;
-  while (parts < kMaxCluster && pairs * parts * 2 <= 148 * PARTS && a.longest > 2 * kSelect * parts) parts *= 2;
+  while (parts < kMaxCluster && pairs * parts * 2 <= 148 * 4 && a.longest > 2 * kSelect * parts) parts *= 2;
   const int rounds = std::max(1, (a.longest + parts * kSelect - 1) / (parts * kSelect));
   const bool fits = rounds * kSelect <= kSelectKeys;
   cudaLaunchAttribute at{};
