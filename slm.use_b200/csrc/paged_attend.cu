@@ -70,7 +70,10 @@ __host__ __device__ inline int visible_of(uint32_t len, long long reach) {
 // at 256).  Measured against 3 CTAs an SM with smaller tiles (us, 64 ragged
 // sequences f32 64 / 48 bf16 128 / 8 x 65536 bf16 128): 45.5 / 167 / 319 so,
 // 44.9 / 178 / 341 with two buffers, 46.1 / 204 / 390 with 8-slot tiles.
-constexpr int kCfg[6][3] = {{16, 3, 2}, {8, 3, 2}, {8, 2, 1}, {32, 3, 2}, {16, 3, 2}, {16, 2, 1}};
+#ifndef C256
+#define C256 {8, 3, 2}
+#endif
+constexpr int kCfg[6][3] = {{16, 3, 2}, {8, 3, 2}, {8, 3, 1}, {32, 3, 2}, {16, 3, 2}, C256};
 template <int SIZE, int DH>
 struct Shape {
   static constexpr int kIndex = (SIZE == 2 ? 3 : 0) + (DH == 64 ? 0 : DH == 128 ? 1 : 2);
@@ -78,9 +81,9 @@ struct Shape {
   static constexpr int kKeys = kCfg[kIndex][0];
   static constexpr int kStages = kCfg[kIndex][1];
   static constexpr int kTile = kKeys * kRow;         // K (or V) bytes of a tile
-  static constexpr bool kQShared = DH > 128;         // q in shared memory: registers hold the sums
-  static constexpr int kWarp = kStages * 2 * kTile + (kQShared ? DH / 8 * 512 : 0);  // bytes of a warp
-  static constexpr int kSmem = kWarps * kWarp;
+  static constexpr int kWarp = kStages * 2 * kTile;  // bytes of a warp's buffers
+  static constexpr bool kQShared = DH > 128;         // q in shared memory, for a CTA: registers hold the sums
+  static constexpr int kSmem = kWarps * kWarp + (kQShared ? DH / 8 * 512 : 0);
   static constexpr int kCtas = kCfg[kIndex][2];
 };
 
@@ -149,12 +152,13 @@ struct Operand<true> {
 // query heads of one key head), has ⌈visible / keys⌉ blocks of `keys` slots.
 // Pairs lie one after the other in units: `extra` (what beginning a pair costs,
 // in blocks) plus its blocks; with whole = true a pair is one unit, never cut.
+// A taker is a warp, or (by_cta) a CTA whose warps take blocks in turn.
 struct Work {
   uint32_t keys, extra;
-  uint32_t takers;              // warps (CTAs if whole) that share the units:
+  uint32_t takers;              // warps (CTAs if by_cta) that share the units:
   uint32_t each, more;          // `each` and one more for the first `more`
   int tiles;                    // pairs of a sequence
-  bool whole;
+  bool whole, by_cta;
   __host__ __device__ uint32_t blocks_of(uint32_t visible) const { return (visible + keys - 1) / keys; }
   __host__ __device__ uint32_t units_of(uint32_t visible) const {  // of a pair
     return visible == 0 ? 0 : whole ? 1 : blocks_of(visible) + extra;
@@ -219,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int group = a.heads / a.key_heads, per_key = (group + kHeads - 1) / kHeads;
   const uint32_t mine = (uint32_t)__cvta_generic_to_shared(smem) + warp * S::kWarp;
-  unsigned char* q_shared = smem + warp * S::kWarp + kStages * 2 * S::kTile;
+  unsigned char* q_shared = smem + kWarps * S::kWarp;
   const uint32_t q_at = (uint32_t)__cvta_generic_to_shared(q_shared) + lane * 16;
   const char *K = static_cast<const char*>(a.k), *V = static_cast<const char*>(a.v);
   const int row_bytes = a.dh * SIZE, pieces = row_bytes / 16;
@@ -229,11 +233,11 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
     for (int i = blockIdx.x; i < a.t.n; i += gridDim.x)
       if (len_of(a.t, lens, i) == 0)
         for (int e = threadIdx.x; e < a.heads * a.dh; e += kThreads) a.y[(size_t)i * a.heads * a.dh + e] = 0.0f;
-  // This taker's units, and where they begin.  Where pairs are whole, a CTA's
-  // warps share them block by block; else every warp is a taker of its own.
-  const uint32_t w = wk.whole ? blockIdx.x : blockIdx.x * kWarps + warp;
+  // This taker's units, and where they begin.
+  const bool by_cta = S::kQShared || wk.by_cta;
+  const uint32_t w = by_cta ? blockIdx.x : blockIdx.x * kWarps + warp;
   if (w >= wk.takers) return;
-  const int turn = wk.whole ? warp : 0, turns = wk.whole ? kWarps : 1;
+  const int turn = by_cta ? warp : 0, turns = by_cta ? kWarps : 1;
   const uint32_t begin = wk.first_unit(w);
   uint32_t left = wk.first_unit(w + 1) - begin;
   Place at = locate(a.t, lens, a.reach, wk, begin);
@@ -309,15 +313,15 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
         split(v[2 * e + 1] * (a.scale * kLog2e), to[2], to[3]);
       };
       if (S::kQShared) {
-#pragma unroll 4
-        for (int i = 0; i < kSteps / kLoad; i++) {
+#pragma unroll
+        for (int i = 0; i < kSteps / kLoad / kWarps; i++) {
           float v[kLoad * 2];
-          read(i, v);
+          read(i * kWarps + warp, v);
 #pragma unroll
           for (int e = 0; e < kLoad; e++) {
             uint32_t to[4];
             parts(v, e, to);
-            *reinterpret_cast<uint4*>(q_shared + (i * kLoad + e) * 512 + lane * 16) =
+            *reinterpret_cast<uint4*>(q_shared + ((i * kWarps + warp) * kLoad + e) * 512 + lane * 16) =
                 make_uint4(to[0], to[1], to[2], to[3]);
           }
         }
@@ -340,6 +344,7 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
       }
     }
 
+    if (S::kQShared) __syncthreads();
     float m = -INFINITY, l = 0.0f, o[kSteps][4];
 #pragma unroll
     for (int s = 0; s < kSteps; s++)
@@ -457,16 +462,16 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
 
-    // The sums of a pair done by this warp alone, of a piece of it, or (a whole
-    // pair of a CTA) of this warp's blocks, to be joined in shared memory.  A
-    // warp cuts at most two pairs, the one it continues and the one it begins.
-    const bool mine_all = !wk.whole && b1 - b0 == n_blocks;
+    // The sums of this taker's share of the pair: all of it, or a piece to be
+    // joined with others (a taker cuts at most two pairs, the one it continues
+    // and the one it begins).  A CTA's warps are joined in shared memory first.
+    const bool all = b1 - b0 == n_blocks;
     const size_t slot = 2 * (size_t)w + (b0 == 0);
-    const float r = mine_all ? 1.0f / l : 1.0f;
-    float* y = a.y + ((size_t)at.seq * a.heads + head0) * a.dh;
-    float* stat = sc.stat ? sc.stat + 2 * ((size_t)at.seq * a.heads + head0) : nullptr;
-    float* sums = reinterpret_cast<float*>(smem + warp * S::kWarp);
-    float* to = wk.whole ? sums + g * kSum : (mine_all ? y : sc.part + slot * kHeads * a.dh) + g * a.dh;
+    const float r = all && !by_cta ? 1.0f / l : 1.0f;
+    float* dst = all ? a.y + ((size_t)at.seq * a.heads + head0) * a.dh : sc.part + slot * kHeads * a.dh;
+    float* ml = !all ? sc.part_ml + slot * kHeads * 2
+                     : sc.stat ? sc.stat + 2 * ((size_t)at.seq * a.heads + head0) : nullptr;
+    float* to = by_cta ? reinterpret_cast<float*>(smem + warp * S::kWarp) + g * kSum : dst + g * a.dh;
     if (g < heads) {
       constexpr int kWide = BF16 ? 8 : 4;  // columns of a 16-byte piece: lane t holds 2 · kWide in a row
 #pragma unroll
@@ -481,21 +486,15 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
             for (int f = 0; f < 4; f++) v[f] = (o[i * kWide + c + f][e] + o[i * kWide + c + f][e + 2]) * r;
             if (d < a.dh) *reinterpret_cast<float4*>(to + d) = make_float4(v[0], v[1], v[2], v[3]);
           }
-      if (t == 0) {
-        if (wk.whole) {
-          s_m[warp][g] = m, s_l[warp][g] = l;
-        } else if (!mine_all) {
-          float* ml = sc.part_ml + (slot * kHeads + g) * 2;
-          ml[0] = m, ml[1] = l;
-        } else if (stat) {
-          stat[2 * g] = m, stat[2 * g + 1] = r;
-        }
-      }
+      if (t == 0 && by_cta)
+        s_m[warp][g] = m, s_l[warp][g] = l;
+      else if (t == 0 && ml)
+        ml[2 * g] = m, ml[2 * g + 1] = all ? r : l;
     }
-    if (wk.whole) {
+    if (by_cta) {
       __syncthreads();
       for (int h = warp; h < heads; h += kWarps) {
-        float M = s_m[0][h], L = 0.0f, f[kWarps];  // warp 0 has a block: M > -inf unless the scores are not finite
+        float M = s_m[0][h], L = 0.0f, f[kWarps];
 #pragma unroll
         for (int x = 1; x < kWarps; x++) M = fmaxf(M, s_m[x][h]);
 #pragma unroll
@@ -503,13 +502,14 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
           f[x] = s_l[x][h] == 0.0f ? 0.0f : exp2_of(s_m[x][h] - M);  // 0: a warp without blocks
           L += s_l[x][h] * f[x];
         }
+        const float norm = all ? 1.0f / L : 1.0f;
         for (int d = lane; d < a.dh; d += 32) {
           float v = 0.0f;
 #pragma unroll
           for (int x = 0; x < kWarps; x++) v += reinterpret_cast<float*>(smem + x * S::kWarp)[h * kSum + d] * f[x];
-          y[h * a.dh + d] = v / L;
+          dst[h * a.dh + d] = v * norm;
         }
-        if (stat && lane == 0) stat[2 * h] = M, stat[2 * h + 1] = 1.0f / L;
+        if (ml && lane == 0) ml[2 * h] = M, ml[2 * h + 1] = all ? norm : L;
       }
       __syncthreads();  // before the next pair's copies
     }
@@ -532,44 +532,70 @@ __device__ __forceinline__ float4 load_if(const float* p, bool ok) {
   return r;
 }
 
+// (M, L) := the maximum and the sum of exp2(x - maximum) of two sets of scores.
+__device__ __forceinline__ void merge(float& M, float& L, float m, float l) {
+  const float to = fmaxf(M, m);
+  L = (M == -INFINITY ? 0.0f : L * exp2_of(M - to)) + (m == -INFINITY ? l : l * exp2_of(m - to));
+  M = to;
+}
+__device__ __forceinline__ void merge_warp(float& M, float& L) {
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) {
+    const float m = __shfl_xor_sync(0xffffffffu, M, x), l = __shfl_xor_sync(0xffffffffu, L, x);
+    merge(M, L, m, l);
+  }
+}
+
+// The pair that holds unit `at` of taker `taker` is cut between w0 and w1.
+struct Pieces {
+  uint32_t w0, w1;
+  // Piece c of head h of the pair: the first taker's second slot, then the others' first ones.
+  __device__ size_t slot_of(int c, int h) const { return (2 * (size_t)(w0 + c) + (c == 0)) * kHeads + h; }
+  __device__ int count() const { return w1 - w0 + 1; }
+};
+__device__ __forceinline__ Pieces pieces_of(const Work& wk, uint32_t origin, uint32_t blocks) {
+  if (wk.whole) return Pieces{0, 0};
+  return Pieces{wk.taker_of(origin + wk.extra), wk.taker_of(origin + wk.extra + blocks - 1)};
+}
+// First unit of a sequence (every warp for itself).
+__device__ __forceinline__ uint32_t first_unit_of(const PagedTable& t, const Lens& lens, long long reach, const Work& wk,
+                                                  int seq) {
+  uint32_t before = 0;
+  for (int i = threadIdx.x & 31; i < seq; i += 32) before += wk.units_of(visible_of(len_of(t, lens, i), reach));
+  return __reduce_add_sync(0xffffffffu, before) * wk.tiles;
+}
+
 // Joins the pieces of cut pairs, a CTA per head of one.  Where there are fewer
-// pairs than warps, blockIdx.x counts them; else it counts the warps, and the
-// first warp of a cut pair joins it.
-constexpr int kMaxWarps = 148 * 2 * kWarps;
+// pairs than takers, `x` counts them; else it counts the takers, and the first
+// taker of a cut pair joins it.
+constexpr int kMaxTakers = 148 * 2 * kWarps;
 template <int kJoin>
-__global__ void __launch_bounds__(kJoin)
-    k_paged_join(const __grid_constant__ PagedAttendArgs a, const __grid_constant__ Scratch sc,
-                 const __grid_constant__ Lens lens, const __grid_constant__ Work wk, bool by_pair) {
-  __shared__ float s_factor[kMaxWarps], s_red[2][kJoin / 32], s_sum[kJoin * 4];
+__device__ void join(const PagedAttendArgs& a, const Scratch& sc, const Lens& lens, const Work& wk, bool by_pair,
+                     uint32_t x0, int y0) {
+  __shared__ float s_factor[kMaxTakers], s_red[2][kJoin / 32], s_sum[kJoin * 4];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = a.heads / a.key_heads, per_key = (group + kHeads - 1) / kHeads;
-  dependents_launch();
   int seq, tile;
   uint32_t origin, n;  // the pair's first unit, and its blocks
   if (by_pair) {
-    seq = blockIdx.x / wk.tiles, tile = blockIdx.x % wk.tiles;
-    uint32_t before = 0;
-    for (int i = lane; i < seq; i += 32) before += wk.units_of(visible_of(len_of(a.t, lens, i), a.reach));
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) before += __shfl_xor_sync(0xffffffffu, before, x);
+    seq = x0 / wk.tiles, tile = x0 % wk.tiles;
     const uint32_t visible = visible_of(len_of(a.t, lens, seq), a.reach);
     n = wk.blocks_of(visible);
-    origin = before * wk.tiles + tile * wk.units_of(visible);
+    origin = first_unit_of(a.t, lens, a.reach, wk, seq) + tile * wk.units_of(visible);
   } else {
-    // The pair that holds the last unit of warp blockIdx.x.
-    const uint32_t at = wk.first_unit(blockIdx.x + 1) - 1;
+    // The pair that holds the last unit of taker x0.
+    const uint32_t at = wk.first_unit(x0 + 1) - 1;
     const Place p = locate(a.t, lens, a.reach, wk, at);
     n = wk.blocks_of(p.visible);
     seq = p.seq, tile = p.unit / wk.units_of(p.visible);
     origin = at - (p.unit - tile * wk.units_of(p.visible));
   }
   dependency_wait();  // every CTA: that this kernel is done says that the one before it is
-  const uint32_t w0 = wk.taker_of(origin + wk.extra), w1 = n ? wk.taker_of(origin + wk.extra + n - 1) : w0;
-  const int kh = tile / per_key, head = tile % per_key * kHeads + blockIdx.y;  // of the key head's
-  if (n == 0 || w0 == w1 || (!by_pair && w0 != blockIdx.x) || head >= group) return;
-  const int parts = w1 - w0 + 1;
-  // Piece c: the first warp's second slot, then the others' first ones.
-  auto slot_of = [&](int c) { return (2 * (size_t)(w0 + c) + (c == 0)) * kHeads + blockIdx.y; };
+  if (n == 0) return;
+  const Pieces pc = pieces_of(wk, origin, n);
+  const int kh = tile / per_key, head = tile % per_key * kHeads + y0;  // of the key head's
+  if (pc.w0 == pc.w1 || (!by_pair && pc.w0 != x0) || head >= group) return;
+  const int parts = pc.count();
 
   // Threads of a group take 4 columns each, groups every so-manieth piece; the
   // first pieces are on their way while the factors are worked out.
@@ -578,28 +604,24 @@ __global__ void __launch_bounds__(kJoin)
   float4 x[kAtOnce], v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   auto fetch = [&](int c) {
 #pragma unroll
-    for (int u = 0; u < kAtOnce; u++) x[u] = load_if(sc.part + slot_of(c + u * groups) * a.dh + d, c + u * groups < parts);
+    for (int u = 0; u < kAtOnce; u++)
+      x[u] = load_if(sc.part + pc.slot_of(c + u * groups, y0) * a.dh + d, c + u * groups < parts);
   };
   fetch(mine);
 
   // M and l of the pieces, and each piece's factor.
   float M = -INFINITY, L = 0.0f;
   for (int c = tid; c < parts; c += kJoin) {
-    const float2 ml = __ldcg(reinterpret_cast<const float2*>(sc.part_ml) + slot_of(c));
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(sc.part_ml) + pc.slot_of(c, y0));
     s_factor[c] = ml.x;
-    const float to = fmaxf(M, ml.x);
-    L = (M == -INFINITY ? 0.0f : L * exp2_of(M - to)) + ml.y * exp2_of(ml.x - to);
-    M = to;
+    merge(M, L, ml.x, ml.y);
   }
-  const float top = warp_max(M);
-  L = warp_sum(M == -INFINITY ? 0.0f : L * exp2_of(M - top));
-  if (lane == 0) s_red[0][warp] = top, s_red[1][warp] = L;
+  merge_warp(M, L);
+  if (lane == 0) s_red[0][warp] = M, s_red[1][warp] = L;
   __syncthreads();
-  M = s_red[0][0], L = 0.0f;
+  M = s_red[0][0], L = s_red[1][0];
 #pragma unroll
-  for (int w = 1; w < kJoin / 32; w++) M = fmaxf(M, s_red[0][w]);
-#pragma unroll
-  for (int w = 0; w < kJoin / 32; w++) L += s_red[0][w] == -INFINITY ? 0.0f : s_red[1][w] * exp2_of(s_red[0][w] - M);
+  for (int w = 1; w < kJoin / 32; w++) merge(M, L, s_red[0][w], s_red[1][w]);
   for (int c = mine;;) {
 #pragma unroll
     for (int u = 0; u < kAtOnce; u++) {
@@ -619,29 +641,77 @@ __global__ void __launch_bounds__(kJoin)
     for (int w = 0; w < groups; w++) sum += s_sum[w * a.dh + e];
     a.y[row * a.dh + e] = sum / L;
   }
-  if (sc.stat && tid == 0) sc.stat[2 * row] = M, sc.stat[2 * row + 1] = 1.0f / L;
 }
 
 // weight[s] += Σ_h p_s over the key head's query heads, from the kept scores:
-// a thread per slot.
-__global__ void __launch_bounds__(kWeightKeys)
-    k_paged_weights(const __grid_constant__ PagedAttendArgs a, const __grid_constant__ Scratch sc,
-                    const __grid_constant__ Lens lens) {
-  const int kh = blockIdx.x % a.key_heads, group = a.heads / a.key_heads;
-  const Place at = locate(a.t, lens, a.reach, Work{kWeightKeys, 0, 0, 0, 0, 1, false}, blockIdx.x / a.key_heads);
-  const int v = at.unit * kWeightKeys + threadIdx.x, padded = (at.visible + 3) & ~3;
-  if (v >= at.visible) return;
-  const uint32_t s = len_of(a.t, lens, at.seq) - at.visible + v, page = a.t.page_of(s);
-  float* w = a.weights + ((size_t)a.t.ids[(size_t)at.seq * a.t.per + page] * a.key_heads + kh) * a.t.page +
-             (s - page * a.t.page);
-  const float was = *w;
+// kWeightKeys slots of one key head and sequence, after M and 1 / l of its
+// heads, kStats at a time, from the pieces or, of a pair that was not cut, as
+// kept.
+constexpr int kStats = 32;
+template <int kThreads_>
+__device__ void add_weights(const PagedAttendArgs& a, const Scratch& sc, const Lens& lens, const Work& wk, uint32_t x0) {
+  __shared__ float s_stat[kStats][2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int kh = x0 % a.key_heads, group = a.heads / a.key_heads, per_key = (group + kHeads - 1) / kHeads;
+  const Place at = locate(a.t, lens, a.reach, Work{kWeightKeys, 0, 0, 0, 0, 1, false, false}, x0 / a.key_heads);
+  const uint32_t n = wk.blocks_of(at.visible), n_units = wk.units_of(at.visible);
+  const uint32_t origin = first_unit_of(a.t, lens, a.reach, wk, at.seq) + kh * per_key * n_units;
+  constexpr int kEach = kWeightKeys / kThreads_;
+  float* w[kEach];
+  float was[kEach], sum[kEach];
+  const int padded = (at.visible + 3) & ~3;
+#pragma unroll
+  for (int e = 0; e < kEach; e++) {
+    const int v = at.unit * kWeightKeys + e * kThreads_ + tid;
+    const uint32_t s = len_of(a.t, lens, at.seq) - at.visible + min(v, at.visible - 1), page = a.t.page_of(s);
+    w[e] = a.weights + ((size_t)a.t.ids[(size_t)at.seq * a.t.per + page] * a.key_heads + kh) * a.t.page +
+           (s - page * a.t.page);
+    was[e] = *w[e], sum[e] = 0.0f;
+  }
   dependency_wait();
-  const float* score = sc.score + at.slots * a.heads + (size_t)kh * group * padded + v;
-  const float* stat = sc.stat + 2 * ((size_t)at.seq * a.heads + kh * group);
-  float sum = 0.0f;
+  const float* score = sc.score + at.slots * a.heads + (size_t)kh * group * padded;
+  for (int h0 = 0; h0 < group; h0 += kStats) {
+    const int count = min(kStats, group - h0);
+    __syncthreads();
+    for (int h = warp; h < count; h += kThreads_ / 32) {
+      const Pieces pc = pieces_of(wk, origin + (h0 + h) / kHeads * n_units, n);
+      const float* stat = sc.stat + 2 * ((size_t)at.seq * a.heads + kh * group + h0 + h);
+      if (pc.w0 == pc.w1) {
+        if (lane < 2) s_stat[h][lane] = __ldcg(stat + lane);
+        continue;
+      }
+      float M = -INFINITY, L = 0.0f;
+      for (int c = lane; c < pc.count(); c += 32) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(sc.part_ml) + pc.slot_of(c, (h0 + h) % kHeads));
+        merge(M, L, ml.x, ml.y);
+      }
+      merge_warp(M, L);
+      if (lane == 0) s_stat[h][0] = M, s_stat[h][1] = 1.0f / L;
+    }
+    __syncthreads();
 #pragma unroll 4
-  for (int h = 0; h < group; h++) sum += exp2_of(score[(size_t)h * padded] - stat[2 * h]) * stat[2 * h + 1];
-  *w = was + sum;
+    for (int h = 0; h < count; h++)
+#pragma unroll
+      for (int e = 0; e < kEach; e++) {
+        const int v = min((int)at.unit * kWeightKeys + e * kThreads_ + tid, at.visible - 1);
+        sum[e] += exp2_of(__ldcg(score + (size_t)(h0 + h) * padded + v) - s_stat[h][0]) * s_stat[h][1];
+      }
+  }
+#pragma unroll
+  for (int e = 0; e < kEach; e++)
+    if ((int)at.unit * kWeightKeys + e * kThreads_ + tid < at.visible) *w[e] = was[e] + sum[e];
+}
+
+// The first `joins` CTAs join (`heads` of them a pair), the others add weights.
+template <int kJoin>
+__global__ void __launch_bounds__(kJoin)
+    k_paged_finish(const __grid_constant__ PagedAttendArgs a, const __grid_constant__ Scratch sc,
+                   const __grid_constant__ Lens lens, const __grid_constant__ Work wk, bool by_pair, uint32_t joins,
+                   uint32_t heads) {
+  if (blockIdx.x < joins)
+    join<kJoin>(a, sc, lens, wk, by_pair, blockIdx.x / heads, blockIdx.x % heads);
+  else
+    add_weights<kJoin>(a, sc, lens, wk, blockIdx.x - joins);
 }
 
 struct Plan {
@@ -662,6 +732,9 @@ constexpr uint32_t kExtra = 2;
 // memory: cut, a call of 97 slots takes 8.2 us instead of 7.7.
 constexpr uint32_t kWholeBlocks = 16;
 
+#ifndef BYCTA
+#define BYCTA 8
+#endif
 Plan plan_of(const PagedAttendArgs& a) {
   Plan p{};
   const int group = a.heads / a.key_heads, dh = padded_dh(a.dh);
@@ -677,7 +750,8 @@ Plan plan_of(const PagedAttendArgs& a) {
   }
   p.idle = busy < (uint32_t)a.t.n;
   wk.whole = wk.blocks_of(longest) <= kWholeBlocks;
-  wk.extra = wk.whole ? 0 : kExtra;
+  wk.by_cta = wk.whole || dh > 128 || wk.tiles * busy * BYCTA <= 148 * cfg[2];
+  wk.extra = wk.whole ? 0 : wk.by_cta ? kExtra * kWarps : kExtra;
   uint64_t units = 0, weight_ctas = 0;
   for (int i = 0; i < a.t.n; i++) {
     const uint32_t v = visible_of(a.host_lens[i], a.reach);
@@ -687,7 +761,7 @@ Plan plan_of(const PagedAttendArgs& a) {
   SLM_REQUIRE(std::max(units, weight_ctas) < (1ull << 31), "paged_attend: too much work for one call");
   p.weight_ctas = (uint32_t)weight_ctas;
   // A taker for every place on the GPU.
-  wk.takers = (uint32_t)std::min<uint64_t>(148 * cfg[2] * (wk.whole ? 1 : kWarps), units);
+  wk.takers = (uint32_t)std::min<uint64_t>(148 * cfg[2] * (wk.by_cta ? 1 : kWarps), units);
   if (wk.takers) wk.each = (uint32_t)(units / wk.takers), wk.more = (uint32_t)(units % wk.takers);
   p.cut = !wk.whole && wk.takers > 1;
   return p;
@@ -714,7 +788,7 @@ size_t carve(const PagedAttendArgs& a, const Plan& p, float* base, Scratch* sc) 
 template <bool BF16, int DH>
 void launch(const PagedAttendArgs& a, const Scratch& sc, const Lens& lens, const Plan& p, cudaStream_t st) {
   const bool q16 = ((uintptr_t)a.q & 15) == 0 && a.ldq % 4 == 0;  // q in 16-byte loads
-  const unsigned ctas = p.work.whole ? p.work.takers : cdiv(p.work.takers, kWarps);
+  const unsigned ctas = p.work.by_cta ? p.work.takers : cdiv(p.work.takers, kWarps);
   k_paged_attend<BF16, DH><<<std::max(1u, ctas), kThreads, Shape<BF16 ? 2 : 4, DH>::kSmem, st>>>(a, sc, lens, p.work,
                                                                                                   p.idle, q16);
 }
@@ -753,17 +827,15 @@ void paged_attend(const PagedAttendArgs& a, cudaStream_t st) {
   else
     (dh == 64 ? launch<false, 64> : dh == 128 ? launch<false, 128> : launch<false, 256>)(a, sc, lens, p, st);
   SLM_LAUNCHED("k_paged_attend");
-  if (p.cut) {
-    const bool by_pair = p.pairs < (int)p.work.takers;
-    const dim3 grid(by_pair ? p.pairs : p.work.takers, std::min(kHeads, a.heads / a.key_heads));
-    // Few pieces a pair: small CTAs, since there are many.
-    if ((int)p.work.takers < 32 * p.pairs && a.dh <= 128)
-      launch_after(k_paged_join<64>, grid, 64, st, a, sc, lens, p.work, by_pair);
-    else
-      launch_after(k_paged_join<256>, grid, 256, st, a, sc, lens, p.work, by_pair);
-  }
-  if (a.weights && p.weight_ctas)
-    launch_after(k_paged_weights, dim3(p.weight_ctas), kWeightKeys, st, a, sc, lens);
+  const bool by_pair = p.pairs < (int)p.work.takers;
+  const uint32_t heads = std::min(kHeads, a.heads / a.key_heads);
+  const uint32_t joins = p.cut ? (by_pair ? p.pairs : p.work.takers) * heads : 0;
+  const uint32_t ctas = joins + (a.weights ? p.weight_ctas : 0);
+  if (!ctas) return;
+  // Few pieces a pair: small CTAs, since there are many.
+  const bool small = (int)p.work.takers < 32 * p.pairs && a.dh <= 128;
+  launch_after(small ? k_paged_finish<64> : k_paged_finish<256>, dim3(ctas), small ? 64 : 256, st, a, sc, lens, p.work,
+               by_pair, joins, heads);
 }
 
 }  // namespace slm
