@@ -9,19 +9,22 @@
 
 namespace slm {
 
-// A kernel may begin while the one before it in the stream still runs: what
-// follows `wait` sees all that the earlier one wrote.
+// The paged kernels begin while the one before them in the stream still runs
+// (launch_after): what follows `dependency_wait` sees all that it wrote.  Every
+// thread block waits, so a kernel is done only after the one before it; and all
+// but the second kernels of a call wait before they let the next one begin, so
+// a second kernel may read what older kernels wrote (the table) at once.
 __device__ __forceinline__ void dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Launches a kernel that begins while the one before it still runs.
 template <class... P, class... A>
-inline void launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, cudaStream_t st, A... args) {
+inline void launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, A... args) {
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t c{};
-  c.gridDim = grid, c.blockDim = dim3(threads), c.stream = st, c.attrs = &at, c.numAttrs = 1;
+  c.gridDim = grid, c.blockDim = dim3(threads), c.dynamicSmemBytes = smem, c.stream = st, c.attrs = &at, c.numAttrs = 1;
   SLM_CUDA(cudaLaunchKernelEx(&c, kernel, P(args)...));
 }
 

@@ -51,16 +51,6 @@ struct Scratch {
   float* score;      // per sequence [heads][visible rounded up to 4], log2 units; or null
 };
 
-// The lengths travel in the launch parameters where they fit (a CTA then finds
-// its place without waiting for memory), else the table's are read.
-constexpr int kLens = 512;
-struct Lens {
-  uint32_t v[kLens];
-};
-__device__ __forceinline__ uint32_t len_of(const PagedTable& t, const Lens& lens, int i) {
-  return t.n <= kLens ? lens.v[i] : t.lens[i];
-}
-
 __host__ __device__ inline int visible_of(uint32_t len, long long reach) {
   return reach && (long long)len > reach ? (int)reach : (int)len;
 }
@@ -159,6 +149,7 @@ struct Work {
   uint32_t each, more;          // `each` and one more for the first `more`
   int tiles;                    // pairs of a sequence
   bool whole, by_cta;
+  bool direct;                  // the sequence of a unit follows from its number: one sequence, or all with `tiles` units
   __host__ __device__ uint32_t blocks_of(uint32_t visible) const { return (visible + keys - 1) / keys; }
   __host__ __device__ uint32_t units_of(uint32_t visible) const {  // of a pair
     return visible == 0 ? 0 : whole ? 1 : blocks_of(visible) + extra;
@@ -173,19 +164,28 @@ struct Work {
 // Finds the sequence that holds unit `at` (every warp for itself) and what lies
 // before it.
 struct Place {
-  int seq, visible;
+  int seq, len, visible;
   uint32_t unit;       // at, counted from the sequence's first unit
   long long slots;     // visible slots of the sequences before it, each rounded up to 4
+  __device__ __forceinline__ void read(const PagedTable& t, long long reach) {
+    len = (int)t.lens[seq];
+    visible = visible_of(len, reach);
+  }
 };
-__device__ __forceinline__ Place locate(const PagedTable& t, const Lens& lens, long long reach, const Work& wk,
-                                        uint32_t at) {
+__device__ __forceinline__ Place locate(const PagedTable& t, long long reach, const Work& wk, uint32_t at) {
+  if (wk.direct) {
+    const int seq = t.n == 1 ? 0 : at / wk.tiles;
+    Place p{seq, 0, 0, at - seq * wk.tiles, 0};
+    p.read(t, reach);
+    return p;
+  }
   const int lane = threadIdx.x & 31, each = (t.n + 31) / 32;
   uint32_t mine = 0;
   long long slots = 0;
 #pragma unroll 4
   for (int j = 0; j < each; j++) {
     const int i = lane * each + j;
-    const uint32_t v = i < t.n ? visible_of(len_of(t, lens, i), reach) : 0;
+    const uint32_t v = i < t.n ? visible_of(t.lens[i], reach) : 0;
     mine += wk.units_of(v) * wk.tiles, slots += (v + 3) & ~3u;
   }
   uint32_t upto = mine;
@@ -197,10 +197,10 @@ __device__ __forceinline__ Place locate(const PagedTable& t, const Lens& lens, l
     if (lane >= o) upto += a, slots_upto += b;
   }
   const int src = __ffs(__ballot_sync(0xffffffffu, upto > at)) - 1;
-  Place p{src * each, 0, at - __shfl_sync(0xffffffffu, upto - mine, src),
+  Place p{src * each, 0, 0, at - __shfl_sync(0xffffffffu, upto - mine, src),
           __shfl_sync(0xffffffffu, slots_upto - slots, src)};
   for (;; p.seq++) {
-    p.visible = visible_of(len_of(t, lens, p.seq), reach);
+    p.read(t, reach);
     const uint32_t n = wk.units_of(p.visible) * wk.tiles;
     if (p.unit < n) return p;
     p.unit -= n, p.slots += (p.visible + 3) & ~3;
@@ -210,7 +210,7 @@ __device__ __forceinline__ Place locate(const PagedTable& t, const Lens& lens, l
 template <bool BF16, int DH>
 __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
     k_paged_attend(const __grid_constant__ PagedAttendArgs a, const __grid_constant__ Scratch sc,
-                   const __grid_constant__ Lens lens, const __grid_constant__ Work wk, bool idle, bool q16) {
+                   const __grid_constant__ Work wk, bool idle, bool q16) {
   constexpr int SIZE = BF16 ? 2 : 4;
   using S = Shape<SIZE, DH>;
   constexpr int kSteps = DH / 8;            // k-steps of q·k, and 8-column tiles of p·v
@@ -228,10 +228,11 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
   const char *K = static_cast<const char*>(a.k), *V = static_cast<const char*>(a.v);
   const int row_bytes = a.dh * SIZE, pieces = row_bytes / 16;
 
+  dependency_wait();
   dependents_launch();
   if (idle)  // rows of idle sequences: zeros
     for (int i = blockIdx.x; i < a.t.n; i += gridDim.x)
-      if (len_of(a.t, lens, i) == 0)
+      if (a.t.lens[i] == 0)
         for (int e = threadIdx.x; e < a.heads * a.dh; e += kThreads) a.y[(size_t)i * a.heads * a.dh + e] = 0.0f;
   // This taker's units, and where they begin.
   const bool by_cta = S::kQShared || wk.by_cta;
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
   const int turn = by_cta ? warp : 0, turns = by_cta ? kWarps : 1;
   const uint32_t begin = wk.first_unit(w);
   uint32_t left = wk.first_unit(w + 1) - begin;
-  Place at = locate(a.t, lens, a.reach, wk, begin);
+  Place at = locate(a.t, a.reach, wk, begin);
 
   while (left) {
     // A segment: blocks b0 .. b1-1 of the pair's n_blocks.
@@ -253,14 +254,14 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
     if (b0 < b1) {
     const int kh = tile / per_key, head0 = kh * group + (tile % per_key) * kHeads;
     const int heads = min(kHeads, (kh + 1) * group - head0);
-    const int lo = (int)len_of(a.t, lens, at.seq) - at.visible;
+    const int lo = at.len - at.visible;
     const int first = lo + b0 * kKeys, end = lo + min((uint32_t)at.visible, b1 * kKeys);
     const uint32_t* ids = a.t.ids + (size_t)at.seq * a.t.per;
     const int n_tiles = ((int)(b1 - b0) - turn + turns - 1) / turns;  // this warp's blocks
     auto key_of = [&](int j) { return first + (j * turns + turn) * kKeys; };
 
     // The pool row that this lane looks up for tile j.
-    auto look_up = [&](int j) -> uint32_t {
+    auto look_up = [&](int j) -> uint32_t {  // j < n_tiles
       const uint32_t s = min(key_of(j) + lane % kKeys, end - 1);
       const uint32_t page = a.t.page_of(s);
       return (ids[page] * a.key_heads + kh) * a.t.page + (s - page * a.t.page);
@@ -286,9 +287,7 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
       }
     };
 
-    uint32_t row[kStages - 1];
-#pragma unroll
-    for (int j = 0; j < kStages - 1; j++) row[j] = j < n_tiles ? look_up(j) : 0;
+    uint32_t row = look_up(0), row1 = n_tiles > 1 ? look_up(1) : 0;  // of the next tiles to load
     // q, scaled to log2 units and split, in the order the key rows are read:
     // rows g and g + 8 of the left operand are head g's hi and lo parts.
     uint32_t qa[S::kQShared ? 1 : kSteps][4];
@@ -329,12 +328,6 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
 #pragma unroll
         for (int i = 0; i < kSteps / kLoad; i++) read(i, qr[S::kQShared ? 0 : i]);
       }
-#pragma unroll
-      for (int j = 0; j < kStages - 1; j++) {
-        if (j < n_tiles) load(j, end - key_of(j), row[j]);
-        copies_commit();
-      }
-      if (kStages - 1 < n_tiles) row[0] = look_up(kStages - 1);
       if (!S::kQShared) {
 #pragma unroll
         for (int i = 0; i < kSteps / kLoad; i++)
@@ -354,15 +347,22 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
                        ? sc.score + at.slots * a.heads + (size_t)(head0 + g) * ((at.visible + 3) & ~3) - lo
                        : nullptr;
 
-    int in = kStages - 1, out = 0;  // buffers
+    int in = 0, out = 0;  // buffers
 #pragma unroll 1
-    for (int j = 0; j < n_tiles; j++) {
-      copies_wait<kStages - 2>();
-      __syncwarp();  // every lane's copies of this tile have landed, and all are done with the last one
-      if (j + kStages - 1 < n_tiles) load(in, end - key_of(j + kStages - 1), row[0]);
+    for (int j = 1 - kStages; j < n_tiles; j++) {
+      if (j >= 0) {
+        copies_wait<kStages - 2>();
+        __syncwarp();  // every lane's copies of this tile have landed, and all are done with the last one
+      }
+      const int next = j + kStages - 1;
+      if (next < n_tiles) {
+        load(in, end - key_of(next), row);
+        row = row1;
+        if (next + 2 < n_tiles) row1 = look_up(next + 2);
+      }
       copies_commit();
-      if (j + kStages < n_tiles) row[0] = look_up(j + kStages);
       in = in + 1 == kStages ? 0 : in + 1;
+      if (j < 0) continue;
 
       const uint32_t kt = mine + out * (2 * S::kTile), vt = kt + S::kTile;
       out = out + 1 == kStages ? 0 : out + 1;
@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
     // On to the next pair or the next sequence with tokens.
     while (left && at.unit >= wk.tiles * wk.units_of(at.visible)) {
       at.unit = 0, at.slots += (at.visible + 3) & ~3;
-      at.visible = visible_of(len_of(a.t, lens, ++at.seq), a.reach);
+      at.seq++, at.read(a.t, a.reach);
     }
   }
 }
@@ -558,10 +558,10 @@ __device__ __forceinline__ Pieces pieces_of(const Work& wk, uint32_t origin, uin
   return Pieces{wk.taker_of(origin + wk.extra), wk.taker_of(origin + wk.extra + blocks - 1)};
 }
 // First unit of a sequence (every warp for itself).
-__device__ __forceinline__ uint32_t first_unit_of(const PagedTable& t, const Lens& lens, long long reach, const Work& wk,
+__device__ __forceinline__ uint32_t first_unit_of(const PagedTable& t, long long reach, const Work& wk,
                                                   int seq) {
   uint32_t before = 0;
-  for (int i = threadIdx.x & 31; i < seq; i += 32) before += wk.units_of(visible_of(len_of(t, lens, i), reach));
+  for (int i = threadIdx.x & 31; i < seq; i += 32) before += wk.units_of(visible_of(t.lens[i], reach));
   return __reduce_add_sync(0xffffffffu, before) * wk.tiles;
 }
 
@@ -570,7 +570,7 @@ __device__ __forceinline__ uint32_t first_unit_of(const PagedTable& t, const Len
 // taker of a cut pair joins it.
 constexpr int kMaxTakers = 148 * 2 * kWarps;
 template <int kJoin>
-__device__ void join(const PagedAttendArgs& a, const Scratch& sc, const Lens& lens, const Work& wk, bool by_pair,
+__device__ void join(const PagedAttendArgs& a, const Scratch& sc, const Work& wk, bool by_pair,
                      uint32_t x0, int y0) {
   __shared__ float s_factor[kMaxTakers], s_red[2][kJoin / 32], s_sum[kJoin * 4];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -579,13 +579,13 @@ __device__ void join(const PagedAttendArgs& a, const Scratch& sc, const Lens& le
   uint32_t origin, n;  // the pair's first unit, and its blocks
   if (by_pair) {
     seq = x0 / wk.tiles, tile = x0 % wk.tiles;
-    const uint32_t visible = visible_of(len_of(a.t, lens, seq), a.reach);
+    const uint32_t visible = visible_of(a.t.lens[seq], a.reach);
     n = wk.blocks_of(visible);
-    origin = first_unit_of(a.t, lens, a.reach, wk, seq) + tile * wk.units_of(visible);
+    origin = first_unit_of(a.t, a.reach, wk, seq) + tile * wk.units_of(visible);
   } else {
     // The pair that holds the last unit of taker x0.
     const uint32_t at = wk.first_unit(x0 + 1) - 1;
-    const Place p = locate(a.t, lens, a.reach, wk, at);
+    const Place p = locate(a.t, a.reach, wk, at);
     n = wk.blocks_of(p.visible);
     seq = p.seq, tile = p.unit / wk.units_of(p.visible);
     origin = at - (p.unit - tile * wk.units_of(p.visible));
@@ -649,13 +649,13 @@ __device__ void join(const PagedAttendArgs& a, const Scratch& sc, const Lens& le
 // kept.
 constexpr int kStats = 32;
 template <int kThreads_>
-__device__ void add_weights(const PagedAttendArgs& a, const Scratch& sc, const Lens& lens, const Work& wk, uint32_t x0) {
+__device__ void add_weights(const PagedAttendArgs& a, const Scratch& sc, const Work& wk, uint32_t x0) {
   __shared__ float s_stat[kStats][2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int kh = x0 % a.key_heads, group = a.heads / a.key_heads, per_key = (group + kHeads - 1) / kHeads;
-  const Place at = locate(a.t, lens, a.reach, Work{kWeightKeys, 0, 0, 0, 0, 1, false, false}, x0 / a.key_heads);
+  const Place at = locate(a.t, a.reach, Work{kWeightKeys, 0, 0, 0, 0, 1, false, false, false}, x0 / a.key_heads);
   const uint32_t n = wk.blocks_of(at.visible), n_units = wk.units_of(at.visible);
-  const uint32_t origin = first_unit_of(a.t, lens, a.reach, wk, at.seq) + kh * per_key * n_units;
+  const uint32_t origin = first_unit_of(a.t, a.reach, wk, at.seq) + kh * per_key * n_units;
   constexpr int kEach = kWeightKeys / kThreads_;
   float* w[kEach];
   float was[kEach], sum[kEach];
@@ -663,7 +663,7 @@ __device__ void add_weights(const PagedAttendArgs& a, const Scratch& sc, const L
 #pragma unroll
   for (int e = 0; e < kEach; e++) {
     const int v = at.unit * kWeightKeys + e * kThreads_ + tid;
-    const uint32_t s = len_of(a.t, lens, at.seq) - at.visible + min(v, at.visible - 1), page = a.t.page_of(s);
+    const uint32_t s = at.len - at.visible + min(v, at.visible - 1), page = a.t.page_of(s);
     w[e] = a.weights + ((size_t)a.t.ids[(size_t)at.seq * a.t.per + page] * a.key_heads + kh) * a.t.page +
            (s - page * a.t.page);
     was[e] = *w[e], sum[e] = 0.0f;
@@ -706,12 +706,12 @@ __device__ void add_weights(const PagedAttendArgs& a, const Scratch& sc, const L
 template <int kJoin>
 __global__ void __launch_bounds__(kJoin)
     k_paged_finish(const __grid_constant__ PagedAttendArgs a, const __grid_constant__ Scratch sc,
-                   const __grid_constant__ Lens lens, const __grid_constant__ Work wk, bool by_pair, uint32_t joins,
+                   const __grid_constant__ Work wk, bool by_pair, uint32_t joins,
                    uint32_t heads) {
   if (blockIdx.x < joins)
-    join<kJoin>(a, sc, lens, wk, by_pair, blockIdx.x / heads, blockIdx.x % heads);
+    join<kJoin>(a, sc, wk, by_pair, blockIdx.x / heads, blockIdx.x % heads);
   else
-    add_weights<kJoin>(a, sc, lens, wk, blockIdx.x - joins);
+    add_weights<kJoin>(a, sc, wk, blockIdx.x - joins);
 }
 
 struct Plan {
@@ -751,6 +751,7 @@ Plan plan_of(const PagedAttendArgs& a) {
   p.idle = busy < (uint32_t)a.t.n;
   wk.whole = wk.blocks_of(longest) <= kWholeBlocks;
   wk.by_cta = wk.whole || dh > 128 || wk.tiles * busy * BYCTA <= 148 * cfg[2];
+  wk.direct = a.t.n == 1 || (wk.whole && !p.idle && !a.weights);
   wk.extra = wk.whole ? 0 : wk.by_cta ? kExtra * kWarps : kExtra;
   uint64_t units = 0, weight_ctas = 0;
   for (int i = 0; i < a.t.n; i++) {
@@ -786,11 +787,11 @@ size_t carve(const PagedAttendArgs& a, const Plan& p, float* base, Scratch* sc) 
 }
 
 template <bool BF16, int DH>
-void launch(const PagedAttendArgs& a, const Scratch& sc, const Lens& lens, const Plan& p, cudaStream_t st) {
+void launch(const PagedAttendArgs& a, const Scratch& sc, const Plan& p, cudaStream_t st) {
   const bool q16 = ((uintptr_t)a.q & 15) == 0 && a.ldq % 4 == 0;  // q in 16-byte loads
   const unsigned ctas = p.work.by_cta ? p.work.takers : cdiv(p.work.takers, kWarps);
-  k_paged_attend<BF16, DH><<<std::max(1u, ctas), kThreads, Shape<BF16 ? 2 : 4, DH>::kSmem, st>>>(a, sc, lens, p.work,
-                                                                                                  p.idle, q16);
+  launch_after(k_paged_attend<BF16, DH>, dim3(std::max(1u, ctas)), kThreads, Shape<BF16 ? 2 : 4, DH>::kSmem, st, a, sc,
+               p.work, p.idle, q16);
 }
 
 template <bool BF16, int DH>
@@ -819,14 +820,11 @@ void paged_attend(const PagedAttendArgs& a, cudaStream_t st) {
   const Plan p = plan_of(a);
   Scratch sc;
   carve(a, p, a.scratch, &sc);
-  Lens lens;
-  if (a.t.n <= kLens) std::copy(a.host_lens, a.host_lens + a.t.n, lens.v);
   const int dh = padded_dh(a.dh);
   if (a.bf16)
-    (dh == 64 ? launch<true, 64> : dh == 128 ? launch<true, 128> : launch<true, 256>)(a, sc, lens, p, st);
+    (dh == 64 ? launch<true, 64> : dh == 128 ? launch<true, 128> : launch<true, 256>)(a, sc, p, st);
   else
-    (dh == 64 ? launch<false, 64> : dh == 128 ? launch<false, 128> : launch<false, 256>)(a, sc, lens, p, st);
-  SLM_LAUNCHED("k_paged_attend");
+    (dh == 64 ? launch<false, 64> : dh == 128 ? launch<false, 128> : launch<false, 256>)(a, sc, p, st);
   const bool by_pair = p.pairs < (int)p.work.takers;
   const uint32_t heads = std::min(kHeads, a.heads / a.key_heads);
   const uint32_t joins = p.cut ? (by_pair ? p.pairs : p.work.takers) * heads : 0;
@@ -834,7 +832,7 @@ void paged_attend(const PagedAttendArgs& a, cudaStream_t st) {
   if (!ctas) return;
   // Few pieces a pair: small CTAs, since there are many.
   const bool small = (int)p.work.takers < 32 * p.pairs && a.dh <= 128;
-  launch_after(small ? k_paged_finish<64> : k_paged_finish<256>, dim3(ctas), small ? 64 : 256, st, a, sc, lens, p.work,
+  launch_after(small ? k_paged_finish<64> : k_paged_finish<256>, dim3(ctas), small ? 64 : 256, 0, st, a, sc, p.work,
                by_pair, joins, heads);
 }
 

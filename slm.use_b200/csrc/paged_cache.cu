@@ -66,6 +66,8 @@ __device__ __forceinline__ void write8(void* pool, size_t at, const float* v) {
 
 template <bool BF16, bool VEC>
 __global__ void __launch_bounds__(kStoreThreads) k_paged_store(const __grid_constant__ PagedStoreArgs a) {
+  dependency_wait();
+  dependents_launch();
   const int lane = threadIdx.x & 31, eights = a.dh / 8, total = a.key_heads * eights;
   const long long tokens = (long long)a.count * a.m, step = (long long)gridDim.x * (kStoreThreads / 32);
   for (long long tok = (long long)blockIdx.x * (kStoreThreads / 32) + (threadIdx.x >> 5); tok < tokens; tok += step) {
@@ -132,9 +134,10 @@ __global__ void __launch_bounds__(kSelect)
   const int parts = cluster.num_blocks(), part = cluster.block_rank();
   const int pair = blockIdx.x / parts, h = pair % a.key_heads, i = pair / a.key_heads;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  dependency_wait();
+  dependents_launch();
   const int n = (int)a.from.lens[i];
   uint32_t* out = a.kept + ((size_t)i * a.key_heads + h) * a.keep;
-  dependents_launch();
   if (n <= a.keep) {  // all kept; uniform in the cluster
     for (int j = part * kSelect + t; j < a.keep; j += parts * kSelect) out[j] = j < n ? (uint32_t)j : 0xffffffffu;
   } else {
@@ -321,11 +324,9 @@ void paged_store(const PagedStoreArgs& a, cudaStream_t st) {
   const bool vec = (((uintptr_t)a.ks | (uintptr_t)a.vs) & 15) == 0 && a.ldk % 4 == 0 && a.ldv % 4 == 0;
   const size_t ctas = ((size_t)a.count * a.m + kStoreThreads / 32 - 1) / (kStoreThreads / 32);
   const unsigned grid = (unsigned)std::min<size_t>(ctas, 148 * 64);
-  if (a.bf16)
-    (vec ? k_paged_store<true, true> : k_paged_store<true, false>)<<<grid, kStoreThreads, 0, st>>>(a);
-  else
-    (vec ? k_paged_store<false, true> : k_paged_store<false, false>)<<<grid, kStoreThreads, 0, st>>>(a);
-  SLM_LAUNCHED("k_paged_store");
+  launch_after(a.bf16 ? (vec ? k_paged_store<true, true> : k_paged_store<true, false>)
+                      : (vec ? k_paged_store<false, true> : k_paged_store<false, false>),
+               dim3(grid), kStoreThreads, 0, st, a);
 }
 
 void paged_evict(const PagedEvictArgs& a, cudaStream_t st) {
@@ -336,19 +337,21 @@ void paged_evict(const PagedEvictArgs& a, cudaStream_t st) {
   while (parts < kMaxCluster && pairs * parts * 2 <= 148 * 4 && a.longest > 2 * kSelect * parts) parts *= 2;
   const int rounds = std::max(1, (a.longest + parts * kSelect - 1) / (parts * kSelect));
   const bool fits = rounds * kSelect <= kSelectKeys;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = (unsigned)parts, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2]{};
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)parts, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t c{};
   c.gridDim = dim3((unsigned)(pairs * parts)), c.blockDim = dim3(kSelect), c.stream = st;
-  c.dynamicSmemBytes = std::min(rounds * kSelect, kSelectKeys) * sizeof(uint32_t), c.attrs = &at, c.numAttrs = 1;
+  c.dynamicSmemBytes = std::min(rounds * kSelect, kSelectKeys) * sizeof(uint32_t), c.attrs = at, c.numAttrs = 2;
   SLM_CUDA(cudaLaunchKernelEx(&c, fits ? k_paged_select<true> : k_paged_select<false>, a));
   const int most = std::min(a.keep, a.longest);
   if (most == 0) return;
   // e / pieces = e · by >> 32 for e < 64 · 64 (one piece: not used).
   const int pieces = a.dh * (a.bf16 ? 2 : 4) / 16, rows = std::min(kMoveRows, std::max(8, 2048 / pieces));
   const uint32_t by = (uint32_t)((((uint64_t)1 << 32) + pieces - 1) / pieces);
-  launch_after(k_paged_move, dim3(cdiv(most, rows), a.key_heads, a.from.n), kMoveThreads, st, a, pieces, by, rows);
+  launch_after(k_paged_move, dim3(cdiv(most, rows), a.key_heads, a.from.n), kMoveThreads, 0, st, a, pieces, by, rows);
 }
 
 }  // namespace slm
