@@ -288,6 +288,16 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
     };
 
     uint32_t row = look_up(0), row1 = n_tiles > 1 ? look_up(1) : 0;  // of the next tiles to load
+    int in = 0, out = 0;  // buffers
+    auto load_next = [&](int next) {
+      if (next < n_tiles) {
+        load(in, end - key_of(next), row);
+        row = row1;
+        if (next + 2 < n_tiles) row1 = look_up(next + 2);
+      }
+      copies_commit();
+      in = in + 1 == kStages ? 0 : in + 1;
+    };
     // q, scaled to log2 units and split, in the order the key rows are read:
     // rows g and g + 8 of the left operand are head g's hi and lo parts.
     uint32_t qa[S::kQShared ? 1 : kSteps][4];
@@ -328,6 +338,8 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
 #pragma unroll
         for (int i = 0; i < kSteps / kLoad; i++) read(i, qr[S::kQShared ? 0 : i]);
       }
+#pragma unroll 1
+    for (int j = 0; j < kStages - 1; j++) load_next(j);
       if (!S::kQShared) {
 #pragma unroll
         for (int i = 0; i < kSteps / kLoad; i++)
@@ -347,22 +359,11 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
                        ? sc.score + at.slots * a.heads + (size_t)(head0 + g) * ((at.visible + 3) & ~3) - lo
                        : nullptr;
 
-    int in = 0, out = 0;  // buffers
 #pragma unroll 1
-    for (int j = 1 - kStages; j < n_tiles; j++) {
-      if (j >= 0) {
-        copies_wait<kStages - 2>();
-        __syncwarp();  // every lane's copies of this tile have landed, and all are done with the last one
-      }
-      const int next = j + kStages - 1;
-      if (next < n_tiles) {
-        load(in, end - key_of(next), row);
-        row = row1;
-        if (next + 2 < n_tiles) row1 = look_up(next + 2);
-      }
-      copies_commit();
-      in = in + 1 == kStages ? 0 : in + 1;
-      if (j < 0) continue;
+    for (int j = 0; j < n_tiles; j++) {
+      copies_wait<kStages - 2>();
+      __syncwarp();  // every lane's copies of this tile have landed, and all are done with the last one
+      load_next(j + kStages - 1);
 
       const uint32_t kt = mine + out * (2 * S::kTile), vt = kt + S::kTile;
       out = out + 1 == kStages ? 0 : out + 1;
@@ -670,6 +671,16 @@ __device__ void add_weights(const PagedAttendArgs& a, const Scratch& sc, const W
   }
   dependency_wait();
   const float* score = sc.score + at.slots * a.heads + (size_t)kh * group * padded;
+  auto score_at = [&](int h, int e) {
+    const int v = min((int)at.unit * kWeightKeys + e * kThreads_ + tid, at.visible - 1);
+    return __ldcg(score + (size_t)h * padded + v);
+  };
+  constexpr int kEarly = 4;  // heads whose scores are read while the statistics are worked out
+  float early[kEarly][kEach];
+#pragma unroll
+  for (int h = 0; h < kEarly; h++)
+#pragma unroll
+    for (int e = 0; e < kEach; e++) early[h][e] = score_at(min(h, group - 1), e);
   for (int h0 = 0; h0 < group; h0 += kStats) {
     const int count = min(kStats, group - h0);
     __syncthreads();
@@ -689,13 +700,18 @@ __device__ void add_weights(const PagedAttendArgs& a, const Scratch& sc, const W
       if (lane == 0) s_stat[h][0] = M, s_stat[h][1] = 1.0f / L;
     }
     __syncthreads();
-#pragma unroll 4
-    for (int h = 0; h < count; h++)
+    int h = 0;
+    if (h0 == 0) {
 #pragma unroll
-      for (int e = 0; e < kEach; e++) {
-        const int v = min((int)at.unit * kWeightKeys + e * kThreads_ + tid, at.visible - 1);
-        sum[e] += exp2_of(__ldcg(score + (size_t)(h0 + h) * padded + v) - s_stat[h][0]) * s_stat[h][1];
-      }
+      for (; h < kEarly; h++)
+        if (h < count)
+#pragma unroll
+          for (int e = 0; e < kEach; e++) sum[e] += exp2_of(early[h][e] - s_stat[h][0]) * s_stat[h][1];
+    }
+#pragma unroll 4
+    for (; h < count; h++)
+#pragma unroll
+      for (int e = 0; e < kEach; e++) sum[e] += exp2_of(score_at(h0 + h, e) - s_stat[h][0]) * s_stat[h][1];
   }
 #pragma unroll
   for (int e = 0; e < kEach; e++)
