@@ -228,9 +228,10 @@ int slm_op_paged_store(slm_ctx* ctx, slm_buf* k, slm_buf* v, slm_buf* weights, s
  * idle row gives zeros.  `scores` is scratch (resized as needed).  With
  * `weights` (null: none) every visible token's weight grows by the sum of its
  * p over the query heads of its key head; fails when two sequences list one
- * page.  Arithmetic is f32 (page values as stored).  Where a query, or a
- * visible key or value, is not finite, that sequence's results are not
- * either or are NaN; slots outside the visible range are not read. */
+ * page.  Arithmetic is f32 or better (page values as stored).  Slots outside
+ * the visible range are not read; where a query, or a visible key or value,
+ * is not finite or their products overflow f32, that sequence's results are
+ * unspecified. */
 int slm_op_paged_attend(slm_ctx* ctx, slm_buf* y, slm_buf* scores, const slm_buf* q, size_t qoff, size_t ldq,
                         const slm_buf* k, const slm_buf* v, slm_buf* weights, slm_table* table, const slm_paged* p);
 /* Brings every sequence of `from` down to at most `keep` tokens per key head,

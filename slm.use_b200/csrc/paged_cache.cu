@@ -92,15 +92,17 @@ __global__ void __launch_bounds__(kStoreThreads) k_paged_store(const __grid_cons
 // ---------------------------------------------------------------------------
 // Evict.  A cluster of CTAs per pair (key head, sequence), each CTA a
 // contiguous slice of its slots with their weights in shared memory, so memory
-// is read once.  The lowest kept weight is found digit by digit from the top
-// (11, 11, 10 bits of an order-preserving integer): every CTA counts its slice,
-// and one warp of each adds the cluster's counts through distributed shared
-// memory, first of 64 digits at a time, then of the 64 that hold the last kept
-// weight.  Latency bounds it.  A second kernel moves the kept tokens' rows,
+// is read once.  The lowest kept weight is found digit by digit from the top of
+// an order-preserving integer: every CTA counts its slice, and one warp of each
+// adds the cluster's counts through distributed shared memory.  Latency bounds
+// it: three digits (11, 11, 10 bits, searched by their upper 5 bits first) in a
+// cluster, where a digit costs a cluster barrier; four of 8 bits in a CTA alone
+// (one of 16640: 14.9 us against 18.7 with four; 32 of 600: 19.1 against 22.3
+// with three).  A second kernel moves the kept tokens' rows,
 // bound by bytes (moved by the searching CTAs themselves, with too few loads in
 // flight, 16 ragged sequences of up to 32768 took 150 us instead of 98).
 // ---------------------------------------------------------------------------
-constexpr int kSelect = 512, kDigits = 2048, kGroup = 64, kMaxCluster = 8;
+constexpr int kSelect = 512, kMaxCluster = 8;
 constexpr int kSelectKeys = 40 * 1024;  // slots of a slice that shared memory holds; longer ones are read again
 constexpr int kSelectWarps = kSelect / 32;
 
@@ -123,15 +125,36 @@ __device__ __forceinline__ int scan_up(int v) {
   return v;
 }
 
-template <bool FITS>
+// Counts `digit` of the lanes that compete; the first one's is likely to be
+// many lanes' (weights share an exponent), so those are counted as one.
+__device__ __forceinline__ void count_digit(int* hist, uint32_t digit, bool competes) {
+  const unsigned lanes = __ballot_sync(0xffffffffu, competes);
+  if (lanes == 0) return;
+  const int leader = __ffs(lanes) - 1, lane = threadIdx.x & 31;
+  const uint32_t most = __shfl_sync(0xffffffffu, digit, leader);
+  const unsigned same = __ballot_sync(0xffffffffu, competes && digit == most);
+  if (lane == leader) atomicAdd(hist + most, __popc(same));
+  if (competes && digit != most) atomicAdd(hist + digit, 1);
+}
+
+// FITS: a slice fits into shared memory; ONE: a CTA a pair, no cluster.
+template <bool FITS, bool ONE>
 __global__ void __launch_bounds__(kSelect)
     k_paged_select(const __grid_constant__ PagedEvictArgs a) {
+  constexpr int kPasses = ONE ? 4 : 3, kDigits = ONE ? 256 : 2048, kCoarse = 32, kGroup = kDigits / kCoarse;
+  constexpr int kTop = ONE ? 24 : 21;  // the lowest bit of the first digit
   extern __shared__ uint32_t s_order[];
-  __shared__ __align__(8) int s_hist[3][kDigits];
-  __shared__ int s_coarse[3][kDigits / kGroup];
+  __shared__ __align__(16) int s_hist[kPasses][kDigits];
+  __shared__ int s_coarse[kPasses][kCoarse];
   __shared__ int s_digit, s_left, s_sure[kSelectWarps + 1], s_tie[kSelectWarps + 1];
   cg::cluster_group cluster = cg::this_cluster();
-  const int parts = cluster.num_blocks(), part = cluster.block_rank();
+  const int parts = ONE ? 1 : cluster.num_blocks(), part = ONE ? 0 : cluster.block_rank();
+  auto sync = [&] {
+    if (ONE)
+      __syncthreads();
+    else
+      cluster.sync();
+  };
   const int pair = blockIdx.x / parts, h = pair % a.key_heads, i = pair / a.key_heads;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   dependency_wait();
@@ -141,19 +164,16 @@ __global__ void __launch_bounds__(kSelect)
   if (n <= a.keep) {  // all kept; uniform in the cluster
     for (int j = part * kSelect + t; j < a.keep; j += parts * kSelect) out[j] = j < n ? (uint32_t)j : 0xffffffffu;
   } else {
-    for (int d = t; d < 3 * kDigits; d += kSelect) (&s_hist[0][0])[d] = 0;
+    for (int d = t; d < kPasses * kDigits; d += kSelect) (&s_hist[0][0])[d] = 0;
     // A warp's slots lie together: 32 · rounds of them.
     const int rounds = (n + parts * kSelect - 1) / (parts * kSelect);
     const int slice = part * rounds * kSelect, mine = warp * rounds * 32 + lane;
     const int lo = a.sinks, hi = n - a.recent;  // the slots that compete
-    auto fetch = [&](int j) -> uint32_t {       // j: in the slice
-      const int s = slice + j;
+    auto order_at = [&](int r) -> uint32_t {
+      const int j = mine + r * 32, s = slice + j;
+      if (FITS || j < kSelectKeys) return s_order[j];
       if (s >= n) return 0;
       return s < lo || s >= hi ? kHeld : order_of(a.weights[pool_row(a.from, i, s, h, a.key_heads)]);
-    };
-    auto order_at = [&](int r) -> uint32_t {
-      const int j = mine + r * 32;
-      return FITS || j < kSelectKeys ? s_order[j] : fetch(j);
     };
     __syncthreads();
     // Several slots' page ids, then weights, on their way at once.
@@ -175,33 +195,57 @@ __global__ void __launch_bounds__(kSelect)
         if (r0 + u >= rounds) break;
         const uint32_t o = s >= n ? 0 : s < lo || s >= hi ? kHeld : order_of(w[u]);
         if (FITS || j < kSelectKeys) s_order[j] = o;
-        if (o != 0 && o != kHeld) atomicAdd(&s_hist[0][o >> 21], 1);
+        const bool competes = o != 0 && o != kHeld;
+        if (ONE)
+          count_digit(s_hist[0], o >> kTop, competes);
+        else if (competes)
+          atomicAdd(&s_hist[0][o >> kTop], 1);
       }
     }
     uint32_t prefix = 0;
     int need = a.keep - a.sinks - a.recent;  // how many of those that compete are kept
     if (need == 0) prefix = kHeld - 1;
-#pragma unroll
-    for (int pass = 0; pass < 3; pass++) {
+#pragma unroll 1
+    for (int pass = 0; pass < kPasses; pass++) {
       if (need == 0) break;  // uniform in the cluster
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+      const int shift = ONE ? 24 - 8 * pass : pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const int bits = ONE ? 8 : pass == 2 ? 10 : 11;
+      int* hist = s_hist[pass];
       if (pass > 0) {
 #pragma unroll 4
         for (int r = 0; r < rounds; r++) {
           const uint32_t o = order_at(r);
-          if (o >> (shift + bits) == prefix >> (shift + bits)) atomicAdd(&s_hist[pass][(o >> shift) & ((1 << bits) - 1)], 1);
+          // The held ones (all bits set) share no prefix with a weight that competes.
+          if ((o ^ prefix) >> (shift + bits) == 0) atomicAdd(hist + (o >> shift & ((1 << bits) - 1)), 1);
         }
       }
-      __syncthreads();
-      // Counts of 64 digits at a time: coarse digit c of this CTA.
-      for (int c = warp; c < kDigits / kGroup; c += kSelectWarps) {
-        const int v = __reduce_add_sync(0xffffffffu, s_hist[pass][c * kGroup + lane] + s_hist[pass][c * kGroup + 32 + lane]);
-        if (lane == 0) s_coarse[pass][c] = v;
+      if (!ONE) {
+        // Counts of kGroup digits at a time.
+        __syncthreads();
+        for (int c = warp; c < kCoarse; c += kSelectWarps) {
+          const int v = __reduce_add_sync(0xffffffffu, hist[c * kGroup + lane] + hist[c * kGroup + kGroup / 2 + lane]);
+          if (lane == 0) s_coarse[pass][c] = v;
+        }
       }
-      cluster.sync();
-      if (warp == 0) {
-        // From the top: the coarse digit that holds the need-th largest, then
-        // the digit, lane by lane two of them.
+      sync();
+      if (warp == 0 && ONE) {
+        // The digit, from the top, that holds the need-th largest: eight of them a lane.
+        const int low = kDigits - 8 - 8 * lane;
+        const int4 x = *reinterpret_cast<const int4*>(hist + low), y = *reinterpret_cast<const int4*>(hist + low + 4);
+        const int c[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        int all = 0;
+#pragma unroll
+        for (int d = 0; d < 8; d++) all += c[d];
+        const int upto = scan_up(all);
+        if (lane == __ffs(__ballot_sync(0xffffffffu, upto >= need)) - 1) {
+          int left = need - (upto - all), digit = low + 7;  // after the digits above this lane's
+#pragma unroll
+          for (int d = 7; d > 0; d--)
+            if (digit == low + d && c[d] < left) left -= c[d], digit--;
+          s_digit = digit, s_left = left;
+        }
+      } else if (warp == 0) {
+        // The group of digits, then the digit, two of them a lane.
         int c = 0;
 #pragma unroll
         for (int p = 0; p < kMaxCluster; p++)
@@ -214,7 +258,7 @@ __global__ void __launch_bounds__(kSelect)
 #pragma unroll
         for (int p = 0; p < kMaxCluster; p++)
           if (p < parts) {
-            const int2 v = *reinterpret_cast<const int2*>(cluster.map_shared_rank(s_hist[pass], p) + top);
+            const int2 v = *reinterpret_cast<const int2*>(cluster.map_shared_rank(hist, p) + top);
             both.x += v.x, both.y += v.y;
           }
         upto = scan_up(both.x + both.y);
@@ -244,7 +288,7 @@ __global__ void __launch_bounds__(kSelect)
       if (lane < kSelectWarps) s_sure[lane] = a0 - a1, s_tie[lane] = b0 - b1;
       if (lane == 31) s_sure[kSelectWarps] = a0, s_tie[kSelectWarps] = b0;
     }
-    cluster.sync();
+    sync();
     sure = s_sure[warp], tie = s_tie[warp];
     for (int p = 0; p < part; p++) {
       sure += cluster.map_shared_rank(s_sure, p)[kSelectWarps];
@@ -261,7 +305,7 @@ __global__ void __launch_bounds__(kSelect)
       sure += __popc(sures), tie += __popc(ties);
     }
   }
-  cluster.sync();  // no CTA leaves while others read its shared memory
+  if (!ONE) cluster.sync();  // no CTA leaves while others read its shared memory
 }
 
 // Moves `rows` kept tokens of a pair: K, V and weight rows in 16-byte pieces
@@ -308,7 +352,8 @@ __global__ void __launch_bounds__(kMoveThreads)
 
 void paged_cache_prepare() {
   const int bytes = kSelectKeys * (int)sizeof(uint32_t);
-  for (auto k : {k_paged_select<false>, k_paged_select<true>})
+  for (auto k : {k_paged_select<false, false>, k_paged_select<false, true>, k_paged_select<true, false>,
+                 k_paged_select<true, true>})
     SLM_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
 }
 
@@ -345,7 +390,9 @@ void paged_evict(const PagedEvictArgs& a, cudaStream_t st) {
   cudaLaunchConfig_t c{};
   c.gridDim = dim3((unsigned)(pairs * parts)), c.blockDim = dim3(kSelect), c.stream = st;
   c.dynamicSmemBytes = std::min(rounds * kSelect, kSelectKeys) * sizeof(uint32_t), c.attrs = at, c.numAttrs = 2;
-  SLM_CUDA(cudaLaunchKernelEx(&c, fits ? k_paged_select<true> : k_paged_select<false>, a));
+  auto select = parts == 1 ? (fits ? k_paged_select<true, true> : k_paged_select<false, true>)
+                           : (fits ? k_paged_select<true, false> : k_paged_select<false, false>);
+  SLM_CUDA(cudaLaunchKernelEx(&c, select, a));
   const int most = std::min(a.keep, a.longest);
   if (most == 0) return;
   // e / pieces = e · by >> 32 for e < 64 · 64 (one piece: not used).
