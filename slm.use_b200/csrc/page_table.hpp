@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <stdexcept>
 #include <string>
+#include <utility>
 #include <vector>
 
 namespace slm {
@@ -53,35 +54,44 @@ class PageTable {
   std::vector<uint32_t> uses;  // sequences that list each page
   std::vector<uint64_t> listed;  // a bit per page: listed by any
   size_t shared = 0;           // pages listed by more than one
-  size_t lo = 0, hi = 0;       // words changed since settle()
+  // Ranges of words set since settle() (they may overlap).
+  std::vector<std::pair<size_t, size_t>> changed;
 
   uint32_t len(size_t i) const { return words[i]; }
   const uint32_t* ids(size_t i) const { return words.data() + seqs + i * per; }
-  void settle() { lo = hi = 0; }
+  void settle() { changed.clear(); }
 
   void assign(size_t seq, const uint32_t* list, size_t n) {
     table_require(list || n == 0, "table_assign: bad arguments");
     table_require(seq < seqs, "table_assign: no such sequence");
     table_require(n <= per, "table_assign: more pages than the table has room for");
     table_require(len(seq) <= n * page, "table_assign: the pages do not hold the sequence's length");
-    std::vector<uint32_t> sorted(list, list + n);
-    std::sort(sorted.begin(), sorted.end());
-    table_require(n == 0 || sorted.back() < pages, "table_assign: page id out of range");
-    table_require(std::adjacent_find(sorted.begin(), sorted.end()) == sorted.end(),
-                  "table_assign: a page comes twice in one sequence");
     uint32_t* row = words.data() + seqs + seq * per;
-    for (size_t j = 0; j < held[seq]; j++) {
+    size_t same = 0;  // a sequence that grew keeps its first pages
+    while (same < n && same < held[seq] && row[same] == list[same]) same++;
+    if (same == held[seq] && n - same <= 8) {  // a few pages more (a step of decoding): no sort
+      for (size_t j = same; j < n; j++) {
+        table_require(list[j] < pages, "table_assign: page id out of range");
+        const uint32_t* from = uses[list[j]] ? list : list + same;  // listed by nobody: only here
+        table_require(std::find(from, list + j, list[j]) == list + j, "table_assign: a page comes twice in one sequence");
+      }
+    } else {
+      std::vector<uint32_t> sorted(list, list + n);
+      std::sort(sorted.begin(), sorted.end());
+      table_require(n == 0 || sorted.back() < pages, "table_assign: page id out of range");
+      table_require(std::adjacent_find(sorted.begin(), sorted.end()) == sorted.end(),
+                    "table_assign: a page comes twice in one sequence");
+    }
+    for (size_t j = same; j < held[seq]; j++) {
       const uint32_t id = row[j], left = --uses[id];
       shared -= left == 1;
       if (left == 0) listed[id / 64] &= ~((uint64_t)1 << id % 64);
     }
-    for (size_t j = 0; j < n; j++) {
+    for (size_t j = same; j < n; j++) {
       const uint32_t id = list[j];
       shared += ++uses[id] == 2;
       listed[id / 64] |= (uint64_t)1 << id % 64;
     }
-    size_t same = 0;  // a sequence that grew keeps its first pages
-    while (same < n && same < held[seq] && row[same] == list[same]) same++;
     std::copy(list + same, list + n, row + same);
     held[seq] = (uint32_t)n;
     if (same < n) touch(seqs + seq * per + same, seqs + seq * per + n);
@@ -130,8 +140,15 @@ class PageTable {
 
  private:
   void touch(size_t a, size_t b) {
-    if (lo == hi) lo = a, hi = b;
-    lo = std::min(lo, a), hi = std::max(hi, b);
+    if (!changed.empty() && changed.back().second == a)
+      changed.back().second = b;
+    else
+      changed.emplace_back(a, b);
+    if (changed.size() > 4096) {  // nobody has looked for long: one range for all
+      size_t lo = words.size(), hi = 0;
+      for (const auto& c : changed) lo = std::min(lo, c.first), hi = std::max(hi, c.second);
+      changed.assign(1, {lo, hi});
+    }
   }
 };
 

@@ -26,19 +26,25 @@ namespace {
 // many as one copy.
 void flush(slm_table* t) {
   PageTable& h = t->host;
-  if (h.lo == h.hi) return;
+  if (h.changed.empty()) return;
+  constexpr size_t kFew = 4 * kPutWords;
   std::vector<uint32_t> at, value;
-  for (size_t i = h.lo; i < h.hi && at.size() <= 4 * kPutWords; i++)
-    if (h.words[i] != t->sent[i]) at.push_back((uint32_t)i), value.push_back(h.words[i]);
+  for (const auto& c : h.changed)
+    for (size_t i = c.first; i < c.second && at.size() <= kFew; i++)
+      if (h.words[i] != t->sent[i]) at.push_back((uint32_t)i), value.push_back(h.words[i]);
   cudaStream_t st = t->ctx->stream;
-  if (at.size() <= 4 * kPutWords)
+  if (at.size() <= kFew) {
     for (size_t j = 0; j < at.size(); j += kPutWords)
       table_put(t->dev, at.data() + j, value.data() + j, (int)std::min<size_t>(kPutWords, at.size() - j), st);
-  else
+    for (size_t j = 0; j < at.size(); j++) t->sent[at[j]] = value[j];
+  } else {
+    size_t lo = h.words.size(), hi = 0;
+    for (const auto& c : h.changed) lo = std::min(lo, c.first), hi = std::max(hi, c.second);
     // Pageable source: the runtime has read it when the call returns.
-    SLM_CUDA(cudaMemcpyAsync(t->dev + h.lo, h.words.data() + h.lo, (h.hi - h.lo) * sizeof(uint32_t),
-                             cudaMemcpyHostToDevice, st));
-  std::copy(h.words.begin() + h.lo, h.words.begin() + h.hi, t->sent.begin() + h.lo);
+    SLM_CUDA(cudaMemcpyAsync(t->dev + lo, h.words.data() + lo, (hi - lo) * sizeof(uint32_t), cudaMemcpyHostToDevice,
+                             st));
+    std::copy(h.words.begin() + lo, h.words.begin() + hi, t->sent.begin() + lo);
+  }
   h.settle();
 }
 

@@ -14,10 +14,10 @@
 // so results do not depend on timing.  Where all pairs are short, a CTA's four
 // warps share one and join it themselves.
 //
-// Data: a warp streams its tiles through three private buffers with 16-byte
-// asynchronous copies, which look every row's page up (a page may end
+// Data: a warp streams its tiles through two or three private buffers with
+// 16-byte asynchronous copies, which look every row's page up (a page may end
 // anywhere in a tile) and fill rows past the end and columns past the head
-// size with zeros.  8 warps an SM keep 128 KB or so in flight.
+// size with zeros.  8 to 12 warps an SM keep about 100 KB in flight.
 //
 // Products: mma.m16n8k8 on tf32, with the group's heads as rows.  Operands of
 // f32 precision are split into two tf32 parts, x = hi + lo: of the 16 rows, 8
@@ -56,14 +56,13 @@ __host__ __device__ inline int visible_of(uint32_t len, long long reach) {
 }
 
 // Slots of a warp's tile, its buffers, and CTAs an SM, for pages of f32 and of
-// bf16 and head sizes up to 64, 128, 256: K and V of a tile take 8 KB (16 KB
-// at 256).  Measured against 3 CTAs an SM with smaller tiles (us, 64 ragged
-// sequences f32 64 / 48 bf16 128 / 8 x 65536 bf16 128): 45.5 / 167 / 319 so,
-// 44.9 / 178 / 341 with two buffers, 46.1 / 204 / 390 with 8-slot tiles.
-#ifndef C256
-#define C256 {8, 3, 2}
-#endif
-constexpr int kCfg[6][3] = {{16, 3, 2}, {8, 3, 2}, {8, 3, 1}, {32, 3, 2}, {16, 3, 2}, C256};
+// bf16 and head sizes up to 64, 128, 256: K and V of a tile take 8 KB (16 KB at
+// f32 256).  Measured (us): at 64, three CTAs with two buffers against two with
+// three, 37.5 / 38.5 for 64 ragged f32 sequences and 13.4 / 14.7 for one of
+// 16389; at 128, where three CTAs leave 168 registers, two against three, 172 /
+// 175 for 48 ragged bf16 sequences; 8-slot tiles at bf16 128, 187.
+constexpr int kCfg[6][3] = {{16, 2, 3}, {8, 3, 2}, {8, 2, 1}, {32, 2, 3}, {16, 3, 2}, {8, 2, 2}};
+constexpr int kMaxCtas = 3;
 template <int SIZE, int DH>
 struct Shape {
   static constexpr int kIndex = (SIZE == 2 ? 3 : 0) + (DH == 64 ? 0 : DH == 128 ? 1 : 2);
@@ -75,6 +74,7 @@ struct Shape {
   static constexpr bool kQShared = DH > 128;         // q in shared memory, for a CTA: registers hold the sums
   static constexpr int kSmem = kWarps * kWarp + (kQShared ? DH / 8 * 512 : 0);
   static constexpr int kCtas = kCfg[kIndex][2];
+  static_assert(kCtas <= kMaxCtas, "more takers than join() has factors for");
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const char* src) {
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
         for (int i = 0; i < kSteps / kLoad; i++) read(i, qr[S::kQShared ? 0 : i]);
       }
 #pragma unroll 1
-    for (int j = 0; j < kStages - 1; j++) load_next(j);
+      for (int j = 0; j < kStages - 1; j++) load_next(j);
       if (!S::kQShared) {
 #pragma unroll
         for (int i = 0; i < kSteps / kLoad; i++)
@@ -351,11 +351,9 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
     }
 
     if (S::kQShared) __syncthreads();
-    float m = -INFINITY, l = 0.0f, o[kSteps][4];
+    float m = -INFINITY, l = 0.0f, o[kSteps][2];
 #pragma unroll
-    for (int s = 0; s < kSteps; s++)
-#pragma unroll
-      for (int j = 0; j < 4; j++) o[s][j] = 0.0f;
+    for (int s = 0; s < kSteps; s++) o[s][0] = o[s][1] = 0.0f;
     float* score = sc.score && g < heads
                        ? sc.score + at.slots * a.heads + (size_t)(head0 + g) * ((at.visible + 3) & ~3) - lo
                        : nullptr;
@@ -432,9 +430,7 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
         const float keep = to == m ? 1.0f : exp2_of(m - to);
         m = to, l *= keep;
 #pragma unroll
-        for (int s = 0; s < kSteps; s++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) o[s][e] *= keep;
+        for (int s = 0; s < kSteps; s++) o[s][0] *= keep, o[s][1] *= keep;
       }
       uint32_t p[kBlocks][4];
 #pragma unroll
@@ -468,10 +464,10 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
             }
           }
         }
+        // The rows' hi and lo parts of a head are added here.
 #pragma unroll
         for (int e = 0; e < kOf; e++)
-#pragma unroll
-          for (int x = 0; x < 4; x++) o[i * kOf + e][x] += f[e][x];
+          o[i * kOf + e][0] += f[e][0] + f[e][2], o[i * kOf + e][1] += f[e][1] + f[e][3];
       }
     }
     __syncwarp();  // all lanes are done with the buffers
@@ -499,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
             const int d = i * (kWide * 8) + (2 * t + e) * kWide + c;
             float v[4];
 #pragma unroll
-            for (int f = 0; f < 4; f++) v[f] = (o[i * kWide + c + f][e] + o[i * kWide + c + f][e + 2]) * r;
+            for (int f = 0; f < 4; f++) v[f] = o[i * kWide + c + f][e] * r;
             if (d < a.dh) *reinterpret_cast<float4*>(to + d) = make_float4(v[0], v[1], v[2], v[3]);
           }
       if (t == 0 && by_cta)
@@ -584,7 +580,7 @@ __device__ __forceinline__ uint32_t first_unit_of(const PagedTable& t, long long
 // Joins the pieces of cut pairs, a CTA per head of one.  Where there are fewer
 // pairs than takers, `x` counts them; else it counts the takers, and the first
 // taker of a cut pair joins it.
-constexpr int kMaxTakers = 148 * 2 * kWarps;
+constexpr int kMaxTakers = 148 * kMaxCtas * kWarps;  // and pieces of a pair
 template <int kJoin>
 __device__ void join(const PagedAttendArgs& a, const Scratch& sc, const Work& wk, bool by_pair,
                      uint32_t x0, int y0) {
@@ -763,9 +759,11 @@ constexpr uint32_t kExtra = 2;
 // memory: cut, a call of 97 slots takes 8.2 us instead of 7.7.
 constexpr uint32_t kWholeBlocks = 16;
 
-#ifndef BYCTA
-#define BYCTA 8
-#endif
+// Where a pair would be cut into more than this many pieces by CTAs, CTAs are
+// the takers (a quarter of the pieces to join): one of 16389 slots 14.0 us
+// against 17.7.
+constexpr uint32_t kManyPieces = 8;
+
 Plan plan_of(const PagedAttendArgs& a) {
   Plan p{};
   const int group = a.heads / a.key_heads, dh = padded_dh(a.dh);
@@ -781,7 +779,7 @@ Plan plan_of(const PagedAttendArgs& a) {
   }
   p.idle = busy < (uint32_t)a.t.n;
   wk.whole = wk.blocks_of(longest) <= kWholeBlocks;
-  wk.by_cta = wk.whole || dh > 128 || wk.tiles * busy * BYCTA <= 148 * cfg[2];
+  wk.by_cta = wk.whole || dh > 128 || wk.tiles * busy * kManyPieces <= 148 * cfg[2];
   wk.direct = a.t.n == 1 || (wk.whole && !p.idle && !a.weights);
   wk.extra = wk.whole ? 0 : wk.by_cta ? kExtra * kWarps : kExtra;
   uint64_t units = 0, weight_ctas = 0;

@@ -40,8 +40,11 @@ int pt_check_evict(void* t, void* to, size_t keep, size_t sinks, size_t recent) 
 }
 size_t pt_shared(void* t) { return at(t)->shared; }
 void pt_words(void* t, uint32_t* out) { std::copy(at(t)->words.begin(), at(t)->words.end(), out); }
+// The words changed since the last call, as first and last ranges' bounds and their number.
 void pt_changed(void* t, size_t* out) {
-  out[0] = at(t)->lo, out[1] = at(t)->hi;
+  out[0] = out[1] = out[2] = 0;
+  const auto& c = at(t)->changed;
+  if (!c.empty()) out[0] = c.front().first, out[1] = c.back().second, out[2] = c.size();
   at(t)->settle();
 }
 }

@@ -142,6 +142,11 @@ ATTEND = [
     ([4500], 12, 4, 64, 16, False, 4096),
     ([6000, 100], 6, 2, 32, 16, False, None),
     ([9, 0, 3000, 77, 1, 2, 500, 499, 64], 8, 8, 64, 64, True, None),
+    ([30000] + [1] * 70, 1, 1, 64, 64, False, None),  # one sequence in pieces of nearly all warps
+    ([30000] + [1] * 70, 2, 1, 64, 64, True, None),
+    ([1 + i % 3 for i in range(700)], 3, 1, 16, 4, False, None),  # more pairs than warps
+    ([(37 * i) % 400 for i in range(300)], 16, 8, 128, 16, True, None),
+    ([(61 * i) % 700 for i in range(200)], 20, 4, 64, 16, False, 333),
 ]
 
 

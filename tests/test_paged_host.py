@@ -67,9 +67,9 @@ class HostTable:
         return a
 
     def changed(self):
-        out = (SZ * 2)()
+        out = (SZ * 3)()
         self.lib.pt_changed(self.h, out)
-        return out[0], out[1]
+        return tuple(out)
 
 
 @pytest.fixture
@@ -111,15 +111,48 @@ def test_only_changed_words_are_marked(table):
     t = table(3, 4, 8, 64)
     t.changed()
     t.assign(1, [5, 6])
-    assert t.changed() == (3 + 4, 3 + 6)
+    assert t.changed() == (3 + 4, 3 + 6, 1)
     t.assign(1, [5, 6, 7])  # a sequence that grew: its new page alone
-    assert t.changed() == (3 + 6, 3 + 7)
+    assert t.changed() == (3 + 6, 3 + 7, 1)
     t.set_lens([0, 17, 0])
-    assert t.changed() == (1, 2)
+    assert t.changed() == (1, 2, 1)
     t.set_lens([0, 17, 0])
-    assert t.changed() == (0, 0)
+    assert t.changed() == (0, 0, 0)
     t.assign(1, [5, 6, 7])
-    assert t.changed() == (0, 0)
+    assert t.changed() == (0, 0, 0)
+    t.set_lens([0, 18, 0])  # a length and a page far behind it: two ranges, not all between
+    t.assign(2, [9])
+    assert t.changed() == (1, 3 + 9, 2)
+
+
+def test_growing_a_sequence_checks_the_new_pages(table):
+    t = table(2, 20, 4, 64)
+    t.assign(0, [1, 2])
+    t.assign(1, [3])
+    for ids in ([1, 2, 2], [1, 2, 1], [1, 2, 5, 5], [1, 2, 64], [1, 2, 5, 6, 5]):
+        with pytest.raises(ValueError):
+            t.assign(0, ids)
+    t.assign(0, [1, 2, 3])  # sequence 1's: shared now
+    assert t.shared == 1
+    t.assign(0, [1, 2, 3, 4])
+    t.assign(0, [1, 2, 3, 4, *range(10, 26)])
+    assert t.shared == 1
+    t.assign(0, [1, 2])
+    assert t.shared == 0
+    t.assign(0, [2, 1])
+    t.set_lens([8, 4])
+    np.testing.assert_array_equal(t.words[2:4], [2, 1])
+
+
+def test_many_small_changes_stay_few_ranges(table):
+    t = table(4096, 1, 1, 4096)
+    for i in range(4096):
+        t.assign(i, [i])
+    t.changed()
+    for step in range(4):  # 2048 ranges of one word each time
+        t.set_lens([i % 2 * ((step + 1) % 2) for i in range(4096)])
+    first, last, ranges = t.changed()
+    assert first <= 1 and last == 4096 and ranges <= 4096
 
 
 def test_shared_pages_are_counted_through_reassignment(table):
