@@ -75,16 +75,16 @@ void own_buffers(slm_ctx* c, std::initializer_list<const slm_buf*> bufs, const c
 // Checks the pool's geometry against the table and its buffers.
 void pool(const slm_paged* p, const slm_table* t, const slm_buf* k, const slm_buf* v, const slm_buf* weights,
           const char* what) {
-  const std::string w(what);
-  SLM_REQUIRE(p->type == SLM_PAGES_F32 || p->type == SLM_PAGES_BF16, w + ": unknown page type");
-  SLM_REQUIRE(p->dh >= 8 && p->dh <= 256 && p->dh % 8 == 0, w + ": head size must be a multiple of 8, at most 256");
-  SLM_REQUIRE(p->key_heads > 0 && p->key_heads <= 65535, w + ": bad number of key heads");
+  auto require = [&](bool ok, const char* msg) { SLM_REQUIRE(ok, std::string(what) + ": " + msg); };
+  require(p->type == SLM_PAGES_F32 || p->type == SLM_PAGES_BF16, "unknown page type");
+  require(p->dh >= 8 && p->dh <= 256 && p->dh % 8 == 0, "head size must be a multiple of 8, at most 256");
+  require(p->key_heads > 0 && p->key_heads <= 65535, "bad number of key heads");
   const size_t rows = checked_mul(checked_mul(t->host.pages, p->key_heads), t->host.page);
-  SLM_REQUIRE(rows < ((size_t)1 << 32), w + ": pages x key heads x page must stay below 2^32");
-  const size_t floats = p->type == SLM_PAGES_BF16 ? checked_mul(rows, p->dh / 2) : checked_mul(rows, p->dh);
-  view(k, 0, floats, (w + " k").c_str());
-  view(v, 0, floats, (w + " v").c_str());
-  if (weights) view(weights, 0, rows, (w + " weights").c_str());
+  require(rows < ((size_t)1 << 32), "pages x key heads x page must stay below 2^32");
+  const size_t floats = p->type == SLM_PAGES_BF16 ? rows * (p->dh / 2) : rows * p->dh;
+  view(k, 0, floats, "paged k");
+  view(v, 0, floats, "paged v");
+  if (weights) view(weights, 0, rows, "paged weights");
 }
 
 // n rows of `width` floats at off, off + ld, …
