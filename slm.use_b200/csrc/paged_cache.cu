@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kSelect)
   constexpr int kHists = ONE ? kPasses : 2;
   __shared__ __align__(16) int s_hist[kHists][kDigits];
   __shared__ int s_coarse[kPasses][kCoarse];
-  __shared__ int s_digit, s_left, s_sure[kSelectWarps + 1], s_tie[kSelectWarps + 1];
+  __shared__ int s_digit, s_left, s_rest, s_sure[kSelectWarps + 1], s_tie[kSelectWarps + 1];
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = ONE ? 1 : cluster.num_blocks(), part = ONE ? 0 : cluster.block_rank();
   auto sync = [&] {
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(kSelect)
 #pragma unroll
           for (int d = 7; d > 0; d--)
             if (digit == low + d && c[d] < left) left -= c[d], digit--;
-          s_digit = digit, s_left = left;
+          s_digit = digit, s_left = left, s_rest = hist[digit] - left;
         }
       } else if (warp == 0) {
         // The group of digits, then the digit, two of them a lane.
@@ -271,12 +271,16 @@ __global__ void __launch_bounds__(kSelect)
         src = __ffs(__ballot_sync(0xffffffffu, upto >= left)) - 1;
         if (lane == src) {
           const int rest = left - (upto - both.x - both.y);  // after the digits above this lane's
-          s_digit = both.y >= rest ? top + 1 : top;
-          s_left = both.y >= rest ? rest : rest - both.y;
+          const bool upper = both.y >= rest;
+          s_digit = upper ? top + 1 : top;
+          s_left = upper ? rest : rest - both.y;
+          s_rest = upper ? both.y - rest : both.x - (rest - both.y);
         }
       }
       __syncthreads();
       prefix |= (uint32_t)s_digit << shift, need = s_left;
+      // All that share the prefix are kept: no more digits are needed.
+      if (s_rest == 0 && prefix != 0) prefix -= 1, need = 0;
     }
     // Above `prefix`: kept; equal to it: the first `need`.  A kept slot's place
     // is the number of sure ones before it and of ties before it, up to `need`.
