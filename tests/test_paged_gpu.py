@@ -169,6 +169,30 @@ def test_attend(slm, ctx, ops, case, weights):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
+def test_attend_at_every_head_size(slm, ctx, ops, bf16):
+    for dh in range(8, 257, 8):
+        rng = np.random.default_rng(dh)
+        group, lens = 1 + dh // 8 % 18, [dh % 37 + 1, 0, 400 + dh]
+        pool = Pool(slm, ctx, ops, rng, lens, 2, dh, 1 + dh % 29, bf16)
+        q = rng.standard_normal((3, 2 * group, dh)).astype(np.float32)
+        y, tol, drawn = pool.formula(q, 2 * group, dh ** -0.5)
+        got = pool.attend(ops.upload(q), 2 * group, dh ** -0.5, weights=True)
+        assert (abs(got - y) <= tol).all(), dh
+        pool.check_weights(pool.w, pool.weights(), drawn)
+
+
+@pytest.mark.parametrize("lens,page", [([1200003], 512), ([i % 5 for i in range(4096)], 2)])
+def test_attend_at_the_ends_of_the_range(slm, ctx, ops, lens, page):
+    rng = np.random.default_rng(17)
+    pool = Pool(slm, ctx, ops, rng, lens, 1, 8, page, True)
+    q = rng.standard_normal((len(lens), 2, 8)).astype(np.float32)
+    y, tol, drawn = pool.formula(q, 2, 0.35)
+    got = pool.attend(ops.upload(q), 2, 0.35, weights=True)
+    assert (abs(got - y) <= tol).all(), float((abs(got - y) / tol).max())
+    pool.check_weights(pool.w, pool.weights(), drawn)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("scale", [3.0, -0.5, 0.0])
 def test_attend_with_peaked_and_flat_scores(slm, ctx, ops, bf16, scale):
     rng = np.random.default_rng(7)
@@ -498,6 +522,49 @@ def test_a_decode_loop_with_a_budget(slm, ctx, ops, bf16):
             tables.reverse()
             np.testing.assert_array_equal(tables[0].lens(), lens)
     assert evictions >= 2
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_queued_calls_do_as_calls_one_by_one(slm, ctx, ops, bf16):
+    """Kernels begin before their predecessors end: a queue of stores, attentions, table changes, other
+    operators and evictions gives the bits of the same calls with a wait after each."""
+    n, heads, kh, dh, page, per = 5, 8, 2, 64, 4, 40
+    pages = 2 * n * per
+    floats = pages * kh * page * dh // (2 if bf16 else 1)
+    args = dict(key_heads=kh, dh=dh, bf16=bf16)
+    results = []
+    for wait in (True, False):
+        rng = np.random.default_rng(44)
+        done = ctx.sync if wait else (lambda: None)
+        kb, vb, wb = ops.zeros(floats), ops.zeros(floats), ops.zeros(pages * kh * page)
+        tables = [slm.Table(ctx, n, per, page, pages) for _ in range(2)]
+        order = rng.permutation(pages).reshape(2, n, per)
+        for t, ids in zip(tables, order):
+            for i in range(n):
+                t.assign(i, ids[i])
+        lens = [100, 7, 0, 130, 64]
+        src = [ops.upload(rng.standard_normal(n * (heads + 2 * kh) * dh)) for _ in range(4)]
+        y, out, scores, kept = ops.zeros(n * heads * dh), ops.zeros(n * heads * dh), ops.zeros(1), ops.zeros(1)
+        ld = (heads + 2 * kh) * dh
+        for step in range(60):
+            lens = [v + (v < per * page) for v in lens]
+            tables[0].set_lens(lens)
+            ops.paged_store(kb, vb, tables[0], (src[step % 4], heads * dh), (src[step % 4], (heads + kh) * dh), m=1,
+                            ldk=ld, ldv=ld, weights=wb, **args)
+            done()
+            ops.paged_attend(y, scores, src[(step + 1) % 4], kb, vb, tables[0], heads=heads, scale=0.125, ldq=ld,
+                             weights=wb if step % 2 else None, **args)
+            done()
+            ops.add(out, out, y, n * heads * dh)
+            done()
+            if step % 7 == 6:
+                ops.paged_evict(kept, kb, vb, wb, tables[0], tables[1], keep=90, sinks=1, recent=8, **args)
+                done()
+                tables.reverse()
+                lens = [min(v, 90) for v in lens]
+        results.append([b.read() for b in (kb, vb, wb, y, out, kept)])
+    for a, b in zip(*results):
+        np.testing.assert_array_equal(a.view(np.uint32), b.view(np.uint32))
 
 
 def test_two_contexts_at_once(slm, ctx, ops):
