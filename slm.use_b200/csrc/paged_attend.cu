@@ -414,10 +414,8 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
           if (s >= end) x[b][0] = -INFINITY;
           if (s + 1 >= end) x[b][1] = -INFINITY;
         }
-        if (score) {
-          if (s < end) score[s] = x[b][0];
-          if (s + 1 < end) score[s + 1] = x[b][1];
-        }
+        // In pairs: rows are padded, and a block ends at an odd slot only at the row's end.
+        if (score && s < end) *reinterpret_cast<float2*>(score + s) = make_float2(x[b][0], x[b][1]);
       }
       float top = x[0][0];
 #pragma unroll
