@@ -55,26 +55,39 @@ __host__ __device__ inline int visible_of(uint32_t len, long long reach) {
   return reach && (long long)len > reach ? (int)reach : (int)len;
 }
 
-// Slots of a warp's tile, its buffers, and CTAs an SM, for pages of f32 and of
-// bf16 and head sizes up to 64, 128, 256: K and V of a tile take 8 KB (16 KB at
-// f32 256).  Measured (us): at 64, three CTAs with two buffers against two with
-// three, 37.5 / 38.5 for 64 ragged f32 sequences and 13.4 / 14.7 for one of
-// 16389; at 128, where three CTAs leave 168 registers, two against three, 172 /
-// 175 for 48 ragged bf16 sequences; 8-slot tiles at bf16 128, 187.
-constexpr int kCfg[6][3] = {{16, 2, 3}, {8, 3, 2}, {8, 2, 1}, {32, 2, 3}, {16, 3, 2}, {8, 2, 2}};
+// Slots of a warp's tile, its buffers, and CTAs an SM, by page type and head
+// size (rounded up to the next one listed: rows in shared memory are multiples
+// of 128 bytes).  K and V of a tile take 6 to 16 KB.  Measured (us): at 64, three
+// CTAs with two buffers against two with three, 37.5 / 38.5 for 64 ragged f32
+// sequences and 13.4 / 14.7 for one of 16389; at 128, where three CTAs leave 168
+// registers, two against three, 172 / 175 for 48 ragged bf16 sequences; 8-slot
+// tiles at bf16 128, 187; f32 96 and 192 by themselves against rounded up to 128
+// and 256, 93 / 105 for 34 sequences of 2393 and 29 / 34 for 8 of 4000.
+struct Config {
+  int dh, keys, stages, ctas;
+};
 constexpr int kMaxCtas = 3;
-template <int SIZE, int DH>
+constexpr Config kF32[] = {{32, 16, 3, 3}, {64, 16, 2, 3}, {96, 8, 3, 3}, {128, 8, 3, 2}, {192, 8, 2, 2}, {256, 8, 2, 1}};
+constexpr Config kBf16[] = {{64, 32, 2, 3}, {128, 16, 3, 2}, {192, 8, 4, 2}, {256, 8, 2, 2}};
+// The first that a head size fits into.
+constexpr Config config_of(bool bf16, int dh) {
+  const Config* c = bf16 ? kBf16 : kF32;
+  while (c->dh < dh) c++;
+  return *c;
+}
+template <bool BF16, int DH>
 struct Shape {
-  static constexpr int kIndex = (SIZE == 2 ? 3 : 0) + (DH == 64 ? 0 : DH == 128 ? 1 : 2);
-  static constexpr int kRow = DH * SIZE;             // bytes of a row in shared memory
-  static constexpr int kKeys = kCfg[kIndex][0];
-  static constexpr int kStages = kCfg[kIndex][1];
+  static constexpr Config kCfg = config_of(BF16, DH);
+  static_assert(kCfg.dh == DH && kCfg.ctas <= kMaxCtas, "configuration");
+  static constexpr int kRow = DH * (BF16 ? 2 : 4);   // bytes of a row in shared memory
+  static constexpr int kKeys = kCfg.keys;
+  static constexpr int kStages = kCfg.stages;
   static constexpr int kTile = kKeys * kRow;         // K (or V) bytes of a tile
   static constexpr int kWarp = kStages * 2 * kTile;  // bytes of a warp's buffers
-  static constexpr bool kQShared = DH > 128;         // q in shared memory, for a CTA: registers hold the sums
+  static constexpr bool kQShared = DH > 192;         // q in shared memory, for a CTA: registers hold the sums
   static constexpr int kSmem = kWarps * kWarp + (kQShared ? DH / 8 * 512 : 0);
-  static constexpr int kCtas = kCfg[kIndex][2];
-  static_assert(kCtas <= kMaxCtas, "more takers than join() has factors for");
+  static constexpr int kCtas = kCfg.ctas;
+  static_assert(kRow % 128 == 0 && kKeys % 8 == 0 && kKeys <= 32, "swizzles and look-ups");
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const char* src) {
@@ -209,11 +222,11 @@ __device__ __forceinline__ Place locate(const PagedTable& t, long long reach, co
 }
 
 template <bool BF16, int DH>
-__global__ void __launch_bounds__(kThreads, Shape<BF16 ? 2 : 4, DH>::kCtas)
+__global__ void __launch_bounds__(kThreads, Shape<BF16, DH>::kCtas)
     k_paged_attend(const __grid_constant__ PagedAttendArgs a, const __grid_constant__ Scratch sc,
                    const __grid_constant__ Work wk, bool idle, bool q16) {
   constexpr int SIZE = BF16 ? 2 : 4;
-  using S = Shape<SIZE, DH>;
+  using S = Shape<BF16, DH>;
   constexpr int kSteps = DH / 8;            // k-steps of q·k, and 8-column tiles of p·v
   constexpr int kLoad = BF16 ? 4 : 2;       // k-steps that a 16-byte piece of a key row feeds
   constexpr int kPieces = S::kRow / 16;     // 16-byte pieces of a row
@@ -747,8 +760,6 @@ struct Plan {
   size_t slots;  // visible slots, each sequence's rounded up to 4
 };
 
-int padded_dh(int dh) { return dh <= 64 ? 64 : dh <= 128 ? 128 : 256; }
-
 // Beginning and ending a pair takes a warp about as long as two blocks (4200
 // cycles against 1900 to 2400 a block): counted so, 16 ragged sequences of 8
 // key heads take 50 us, against 52 at one and 64 without.
@@ -764,10 +775,10 @@ constexpr uint32_t kManyPieces = 8;
 
 Plan plan_of(const PagedAttendArgs& a) {
   Plan p{};
-  const int group = a.heads / a.key_heads, dh = padded_dh(a.dh);
-  const int* cfg = kCfg[(a.bf16 ? 3 : 0) + (dh == 64 ? 0 : dh == 128 ? 1 : 2)];
+  const int group = a.heads / a.key_heads;
+  const Config cfg = config_of(a.bf16, a.dh);
   Work& wk = p.work;
-  wk.keys = cfg[0], wk.tiles = a.key_heads * ((group + kHeads - 1) / kHeads);
+  wk.keys = cfg.keys, wk.tiles = a.key_heads * ((group + kHeads - 1) / kHeads);
   p.pairs = a.t.n * wk.tiles;
   uint32_t longest = 0, busy = 0;
   for (int i = 0; i < a.t.n; i++) {
@@ -777,7 +788,7 @@ Plan plan_of(const PagedAttendArgs& a) {
   }
   p.idle = busy < (uint32_t)a.t.n;
   wk.whole = wk.blocks_of(longest) <= kWholeBlocks;
-  wk.by_cta = wk.whole || dh > 128 || wk.tiles * busy * kManyPieces <= 148 * cfg[2];
+  wk.by_cta = wk.whole || cfg.dh > 192 || wk.tiles * busy * kManyPieces <= 148u * cfg.ctas;
   wk.direct = a.t.n == 1 || (wk.whole && !p.idle && !a.weights);
   wk.extra = wk.whole ? 0 : wk.by_cta ? kExtra * kWarps : kExtra;
   uint64_t units = 0, weight_ctas = 0;
@@ -789,7 +800,7 @@ Plan plan_of(const PagedAttendArgs& a) {
   SLM_REQUIRE(std::max(units, weight_ctas) < (1ull << 31), "paged_attend: too much work for one call");
   p.weight_ctas = (uint32_t)weight_ctas;
   // A taker for every place on the GPU.
-  wk.takers = (uint32_t)std::min<uint64_t>(148 * cfg[2] * (wk.by_cta ? 1 : kWarps), units);
+  wk.takers = (uint32_t)std::min<uint64_t>(148 * cfg.ctas * (wk.by_cta ? 1 : kWarps), units);
   if (wk.takers) wk.each = (uint32_t)(units / wk.takers), wk.more = (uint32_t)(units % wk.takers);
   p.cut = !wk.whole && wk.takers > 1;
   return p;
@@ -817,24 +828,28 @@ template <bool BF16, int DH>
 void launch(const PagedAttendArgs& a, const Scratch& sc, const Plan& p, cudaStream_t st) {
   const bool q16 = ((uintptr_t)a.q & 15) == 0 && a.ldq % 4 == 0;  // q in 16-byte loads
   const unsigned ctas = p.work.by_cta ? p.work.takers : cdiv(p.work.takers, kWarps);
-  launch_after(k_paged_attend<BF16, DH>, dim3(std::max(1u, ctas)), kThreads, Shape<BF16 ? 2 : 4, DH>::kSmem, st, a, sc,
+  launch_after(k_paged_attend<BF16, DH>, dim3(std::max(1u, ctas)), kThreads, Shape<BF16, DH>::kSmem, st, a, sc,
                p.work, p.idle, q16);
 }
 
 template <bool BF16, int DH>
 void prepare() {
   SLM_CUDA(cudaFuncSetAttribute(k_paged_attend<BF16, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                Shape<BF16 ? 2 : 4, DH>::kSmem));
+                                Shape<BF16, DH>::kSmem));
 }
 
 }  // namespace
 
 void paged_prepare() {
+  prepare<false, 32>();
   prepare<false, 64>();
+  prepare<false, 96>();
   prepare<false, 128>();
+  prepare<false, 192>();
   prepare<false, 256>();
   prepare<true, 64>();
   prepare<true, 128>();
+  prepare<true, 192>();
   prepare<true, 256>();
 }
 
@@ -847,11 +862,17 @@ void paged_attend(const PagedAttendArgs& a, cudaStream_t st) {
   const Plan p = plan_of(a);
   Scratch sc;
   carve(a, p, a.scratch, &sc);
-  const int dh = padded_dh(a.dh);
+  const int dh = config_of(a.bf16, a.dh).dh;
   if (a.bf16)
-    (dh == 64 ? launch<true, 64> : dh == 128 ? launch<true, 128> : launch<true, 256>)(a, sc, p, st);
+    (dh == 64 ? launch<true, 64> : dh == 128 ? launch<true, 128> : dh == 192 ? launch<true, 192> : launch<true, 256>)(
+        a, sc, p, st);
   else
-    (dh == 64 ? launch<false, 64> : dh == 128 ? launch<false, 128> : launch<false, 256>)(a, sc, p, st);
+    (dh == 32    ? launch<false, 32>
+     : dh == 64  ? launch<false, 64>
+     : dh == 96  ? launch<false, 96>
+     : dh == 128 ? launch<false, 128>
+     : dh == 192 ? launch<false, 192>
+                 : launch<false, 256>)(a, sc, p, st);
   const bool by_pair = p.pairs < (int)p.work.takers;
   const uint32_t heads = std::min(kHeads, a.heads / a.key_heads);
   const uint32_t joins = p.cut ? (by_pair ? p.pairs : p.work.takers) * heads : 0;
