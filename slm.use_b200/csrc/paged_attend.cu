@@ -808,8 +808,10 @@ Plan plan_of(const PagedAttendArgs& a) {
   }
   SLM_REQUIRE(std::max(units, weight_ctas) < (1ull << 31), "paged_attend: too much work for one call");
   p.weight_ctas = (uint32_t)weight_ctas;
-  // A taker for every place on the GPU.
-  wk.takers = (uint32_t)std::min<uint64_t>(148 * cfg.ctas * (wk.by_cta ? 1 : kWarps), units);
+  // A taker for every place on the GPU; of CTAs at most two an SM, which leaves
+  // room for the second kernel's to be there when the pieces are (one sequence
+  // of 16389 bf16 slots, 64 wide: 9.0 us against 10.4 with three).
+  wk.takers = (uint32_t)std::min<uint64_t>(148 * (wk.by_cta ? std::min(cfg.ctas, 2) : cfg.ctas * kWarps), units);
   if (wk.takers) wk.each = (uint32_t)(units / wk.takers), wk.more = (uint32_t)(units % wk.takers);
   p.cut = !wk.whole && wk.takers > 1;
   return p;
