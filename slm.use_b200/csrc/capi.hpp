@@ -38,7 +38,7 @@ struct slm_ctx {
   void* gemm_ws = nullptr;      // tensor-core GEMM workspace (grown on demand, outside captures)
   size_t gemm_ws_bytes = 0;
   unsigned long long gemm_ws_gen = 0;  // bumped whenever gemm_ws moves (graphs holding it must be re-captured)
-  unsigned* merge_cnt = nullptr;  // attention slice counters of slm_op_attend and slm_op_paged_attend (zero between launches)
+  unsigned* merge_cnt = nullptr;  // attention slice counters of slm_op_attend (zero between launches)
   unsigned* gemv_cnt = nullptr;   // kGemvCounters row-block counters of the split GEMV (zero between launches)
   size_t merge_cnt_len = 0;
   // Live buffers and models of this context.  slm_ctx_free while some live
@@ -82,8 +82,6 @@ void dev_free(void* p);
 void ensure(slm_buf* y, size_t n);
 const float* view(const slm_buf* b, size_t off, size_t n, const char* what);
 void* stage(slm_ctx* c, const void* host, size_t bytes);
-// n of the context's slice counters (zero between launches), grown if needed.
-unsigned* merge_counters(slm_ctx* c, size_t n);
 // Sets a.ws/a.ws_bytes to the context's GEMM workspace, growing it if the
 // tensor-core path needs more (never during a stream capture).
 void gemm_workspace(slm_ctx* c, struct LinearArgs& a, bool capturing);

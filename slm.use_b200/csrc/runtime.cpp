@@ -84,18 +84,6 @@ void* stage(slm_ctx* c, const void* host, size_t bytes) {
   return c->stage;
 }
 
-unsigned* merge_counters(slm_ctx* c, size_t n) {
-  if (c->merge_cnt_len < n) {
-    SLM_CUDA(cudaStreamSynchronize(c->stream));
-    dev_free(c->merge_cnt);
-    c->merge_cnt = nullptr, c->merge_cnt_len = 0;
-    c->merge_cnt = static_cast<unsigned*>(dev_alloc(n * sizeof(unsigned)));
-    SLM_CUDA(cudaMemsetAsync(c->merge_cnt, 0, n * sizeof(unsigned), c->stream));
-    c->merge_cnt_len = n;
-  }
-  return c->merge_cnt;
-}
-
 void gemm_workspace(slm_ctx* c, LinearArgs& a, bool capturing) {
   const bool b3 = b3_linear_ok(a), skinny = !b3 && skinny_ok(a), tc = !skinny && !b3 && a.m > 64 && tc_linear_ok(a);
   const bool gemv = !b3 && !skinny && !tc && a.m <= 8;
@@ -550,9 +538,17 @@ int slm_op_attend(slm_ctx* c, slm_buf* y, slm_buf* scores, const slm_buf* q, siz
       qs = scores->ptr + qat;
     }
     // Counters for merging the slices in the slice launch (kept zero between calls).
-    unsigned* cnt = merge_counters(c, at->m * at->heads);
+    const size_t ncnt = at->m * at->heads;
+    if (c->merge_cnt_len < ncnt) {
+      SLM_CUDA(cudaStreamSynchronize(c->stream));
+      dev_free(c->merge_cnt);
+      c->merge_cnt = nullptr, c->merge_cnt_len = 0;
+      c->merge_cnt = static_cast<unsigned*>(dev_alloc(ncnt * sizeof(unsigned)));
+      SLM_CUDA(cudaMemsetAsync(c->merge_cnt, 0, ncnt * sizeof(unsigned), c->stream));
+      c->merge_cnt_len = ncnt;
+    }
     attention(qs, (int)(at->heads * at->dh), k->ptr, v->ptr, g, nullptr, nsplit, scores->ptr + 2, y->ptr,
-              (int)(at->heads * at->dh), c->stream, cnt);
+              (int)(at->heads * at->dh), c->stream, c->merge_cnt);
   });
 }
 
