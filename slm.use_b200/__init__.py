@@ -4,7 +4,8 @@ A thin ctypes layer over libslm_b200.so (C ABI in include/slm_b200.h).  Names,
 argument meaning and errors follow the reference:
 
   * `Ops` — one method per method of the reference's `Ops` trait
-    (src/ops.rs:68-228) on device buffers (`Buf`);
+    (src/ops.rs:68-228) on device buffers (`Buf`); and, with `Table`, paged
+    key-value caches, which the reference does not have;
   * `Model` / `Session` — Model::load, session, feed, step, logits, state_bytes
     (src/model.rs:225-690);
   * `Sampling`, `rng_seed`, `Session.sample` — pick and Rng (src/sample.rs).
