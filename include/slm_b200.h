@@ -225,7 +225,8 @@ int slm_op_paged_store(slm_ctx* ctx, slm_buf* k, slm_buf* v, slm_buf* weights, s
  * Σ_s p_s v_s over visible slots s, p = softmax of scale · q[i][h]·k_s, with
  * query head h reading key head h / (heads / key_heads).  Row i of q is heads
  * · dh floats at qoff + i·ldq; y is seqs × heads × dh, grown as needed; an
- * idle row gives zeros.  `scores` is scratch (resized as needed).  With
+ * idle row gives zeros.  `scores` is scratch (grown as needed, by a quarter at
+ * least; a call that grows it waits for the calls before it).  With
  * `weights` (null: none) every visible token's weight grows by the sum of its
  * p over the query heads of its key head; fails when two sequences list one
  * page.  Arithmetic is f32 or better (page values as stored).  Slots outside

@@ -207,7 +207,10 @@ int slm_op_paged_attend(slm_ctx* c, slm_buf* y, slm_buf* scores, const slm_buf* 
     a.ldq = (long long)ldq;
     a.k = k->ptr, a.v = v->ptr, a.weights = weights ? weights->ptr : nullptr;
     ensure(y, t->host.seqs * width);
-    ensure(scores, paged_attend_scratch(a));
+    // What the scratch takes grows with the lengths: some more than that, so
+    // that few of a decode loop's steps wait for a new one.
+    const size_t scratch = paged_attend_scratch(a);
+    if (scratch > scores->len) ensure(scores, scratch + scratch / 4);
     a.y = y->ptr, a.scratch = scores->ptr;
     flush(t);
     paged_attend(a, c->stream);

@@ -262,6 +262,24 @@ def test_attend_follows_the_table_in_stream_order(slm, ctx, ops):
     np.testing.assert_array_equal(pool.table.lens(), outs[-1][0])
 
 
+@pytest.mark.parametrize("weights", [False, True])
+def test_scratch_of_a_decode_loop_grows_by_a_quarter_at_least(slm, ctx, ops, weights):
+    """A step that needs more scratch waits for it, so steps that follow are to find some left."""
+    rng = np.random.default_rng(31)
+    pool = Pool(slm, ctx, ops, rng, [640, 500], 2, 64, 16, False)
+    q = rng.standard_normal((2, 6, 64)).astype(np.float32)
+    qb, y, scores, sizes = ops.upload(q), ops.zeros(1), ops.zeros(1), []
+    for step in range(401):
+        pool.table.set_lens([240 + step, 100 + step])
+        ops.paged_attend(y, scores, qb, pool.kb, pool.vb, pool.table, heads=6, key_heads=2, dh=64, scale=0.125,
+                         weights=pool.wb if weights else None)
+        if len(scores) != (sizes or [1])[-1]:
+            sizes.append(len(scores))
+    assert len(sizes) > 1 and all(4 * b >= 5 * a for a, b in zip(sizes, sizes[1:]))
+    want, tol, _ = pool.formula(q, 6, 0.125)
+    assert (abs(y.read().reshape(2, 6, 64) - want) <= tol).all()
+
+
 def test_two_tables_share_a_common_beginning(slm, ctx, ops):
     rng = np.random.default_rng(13)
     pool = Pool(slm, ctx, ops, rng, [50, 20], 2, 64, 16, True, spare=4)
