@@ -46,9 +46,10 @@ constexpr int kWeightKeys = 256;  // slots whose weights a CTA adds at once
 // Where a launch keeps what its warps hand one another.
 struct Scratch {
   float* part;       // [taker][2][heads of a tile][dh]: sums of pieces of cut (sequence, tile)s
-  float* part_ml;    // [taker][2][heads of a tile][2]: their m and l
+  float* part_ml;    // [taker][2][kHeads][2]: their m and l
   float* stat;       // [n][heads][2]: final m and 1 / l, or null
   float* score;      // per sequence [heads][visible rounded up to 4], log2 units; or null
+  uint32_t piece;    // floats of a piece's sums
 };
 
 __host__ __device__ inline int visible_of(uint32_t len, long long reach) {
@@ -487,10 +488,10 @@ __global__ void __launch_bounds__(kThreads, Shape<BF16, DH>::kCtas)
     // joined with others (a taker cuts at most two pairs, the one it continues
     // and the one it begins).  A CTA's warps are joined in shared memory first.
     const bool all = b1 - b0 == n_blocks;
-    const uint32_t slot = (2 * w + (b0 == 0)) * min(kHeads, group);
+    const size_t slot = 2 * (size_t)w + (b0 == 0);
     const float r = all && !by_cta ? 1.0f / l : 1.0f;
-    float* dst = all ? a.y + ((size_t)at.seq * a.heads + head0) * a.dh : sc.part + slot * a.dh;
-    float* ml = !all ? sc.part_ml + slot * 2
+    float* dst = all ? a.y + ((size_t)at.seq * a.heads + head0) * a.dh : sc.part + slot * sc.piece;
+    float* ml = !all ? sc.part_ml + slot * kHeads * 2
                      : sc.stat ? sc.stat + 2 * ((size_t)at.seq * a.heads + head0) : nullptr;
     float* to = by_cta ? reinterpret_cast<float*>(smem + warp * S::kWarp) + g * kSum : dst + g * a.dh;
     if (g < heads) {
@@ -570,15 +571,14 @@ __device__ __forceinline__ void merge_warp(float& M, float& L) {
 // The pair that holds unit `at` of taker `taker` is cut between w0 and w1.
 struct Pieces {
   uint32_t w0, w1;
-  int heads;  // of a tile (a key head's last tile may have fewer)
-  // Piece c of head h of the pair: the first taker's second slot, then the others' first ones.
-  __device__ size_t slot_of(int c, int h) const { return (2 * (size_t)(w0 + c) + (c == 0)) * heads + h; }
+  // Piece c of the pair: the first taker's second slot, then the others' first ones.
+  __device__ size_t slot_of(int c) const { return 2 * (size_t)(w0 + c) + (c == 0); }
+  __device__ size_t slot_of(int c, int h) const { return slot_of(c) * kHeads + h; }
   __device__ int count() const { return w1 - w0 + 1; }
 };
-__device__ __forceinline__ Pieces pieces_of(const Work& wk, int group, uint32_t origin, uint32_t blocks) {
-  const int heads = min(kHeads, group);
-  if (wk.whole) return Pieces{0, 0, heads};
-  return Pieces{wk.taker_of(origin + wk.extra), wk.taker_of(origin + wk.extra + blocks - 1), heads};
+__device__ __forceinline__ Pieces pieces_of(const Work& wk, uint32_t origin, uint32_t blocks) {
+  if (wk.whole) return Pieces{0, 0};
+  return Pieces{wk.taker_of(origin + wk.extra), wk.taker_of(origin + wk.extra + blocks - 1)};
 }
 // First unit of a sequence (every warp for itself).
 __device__ __forceinline__ uint32_t first_unit_of(const PagedTable& t, long long reach, const Work& wk,
@@ -615,7 +615,7 @@ __device__ void join(const PagedAttendArgs& a, const Scratch& sc, const Work& wk
   }
   dependency_wait();  // every CTA: that this kernel is done says that the one before it is
   if (n == 0) return;
-  const Pieces pc = pieces_of(wk, group, origin, n);
+  const Pieces pc = pieces_of(wk, origin, n);
   const int kh = tile / per_key, head = tile % per_key * kHeads + y0;  // of the key head's
   if (pc.w0 == pc.w1 || (!by_pair && pc.w0 != x0) || head >= group) return;
   const int parts = pc.count();
@@ -628,7 +628,7 @@ __device__ void join(const PagedAttendArgs& a, const Scratch& sc, const Work& wk
   auto fetch = [&](int c) {
 #pragma unroll
     for (int u = 0; u < kAtOnce; u++)
-      x[u] = load_if(sc.part + pc.slot_of(c + u * groups, y0) * a.dh + d, c + u * groups < parts);
+      x[u] = load_if(sc.part + pc.slot_of(c + u * groups) * sc.piece + y0 * a.dh + d, c + u * groups < parts);
   };
   fetch(mine);
 
@@ -708,7 +708,7 @@ __device__ void add_weights(const PagedAttendArgs& a, const Scratch& sc, const W
       if (begins || group > kStats) {
         __syncthreads();
         for (int h = warp; h < count; h += kThreads_ / 32) {
-          const Pieces pc = pieces_of(wk, group, origin + (h0 + h) / kHeads * n_units, n);
+          const Pieces pc = pieces_of(wk, origin + (h0 + h) / kHeads * n_units, n);
           const float* stat = sc.stat + 2 * ((size_t)at.seq * a.heads + kh * group + h0 + h);
           if (pc.w0 == pc.w1) {
             if (lane < 2) s_stat[h][lane] = __ldcg(stat + lane);
@@ -827,10 +827,10 @@ size_t carve(const PagedAttendArgs& a, const Plan& p, float* base, Scratch* sc) 
     at += round4(n);
     return r;
   };
-  const size_t pieces = p.cut ? 2 * (size_t)p.work.takers : 0;
-  const size_t heads = std::min(kHeads, a.heads / a.key_heads);
-  sc->part = take(pieces * heads * a.dh);
-  sc->part_ml = take(pieces * heads * 2);
+  const size_t warps = p.cut ? p.work.takers : 0;
+  sc->piece = std::min(kHeads, a.heads / a.key_heads) * a.dh;
+  sc->part = take(2 * warps * sc->piece);
+  sc->part_ml = take(2 * warps * kHeads * 2);
   sc->stat = a.weights ? take((size_t)a.t.n * a.heads * 2) : nullptr;
   sc->score = a.weights ? take(p.slots * a.heads) : nullptr;
   return at + 4;
