@@ -7,6 +7,7 @@
 #include <cstring>
 
 #include "common.cuh"
+#include "evict_order.hpp"
 #include "paged.cuh"
 
 namespace cg = cooperative_groups;
@@ -106,15 +107,6 @@ constexpr int kSelect = 512, kMaxCluster = 8;
 constexpr int kSelectKeys = 40 * 1024;  // slots of a slice that shared memory holds; longer ones are read again
 constexpr int kSelectWarps = kSelect / 32;
 
-// Order of the weights as unsigned integers from 1 on: NaN lowest, the two
-// zeros equal.  0 stands for no slot, kHeld for one that does not compete.
-constexpr uint32_t kHeld = 0xffffffffu;
-__device__ __forceinline__ uint32_t order_of(float w) {
-  if (w != w) return 1;
-  const uint32_t b = __float_as_uint(w + 0.0f);
-  return (b & 0x80000000u ? ~b : b | 0x80000000u) + 1;
-}
-
 // Inclusive sums over the lanes of a warp.
 __device__ __forceinline__ int scan_up(int v) {
 #pragma unroll
@@ -141,8 +133,8 @@ __device__ __forceinline__ void count_digit(int* hist, uint32_t digit, bool comp
 template <bool FITS, bool ONE>
 __global__ void __launch_bounds__(kSelect)
     k_paged_select(const __grid_constant__ PagedEvictArgs a) {
-  constexpr int kPasses = ONE ? 4 : 3, kDigits = ONE ? 256 : 2048, kCoarse = 32, kGroup = kDigits / kCoarse;
-  constexpr int kTop = ONE ? 24 : 21;  // the lowest bit of the first digit
+  using D = Digits<ONE>;
+  constexpr int kPasses = D::kPasses, kDigits = D::kCount, kTop = D::kTop, kCoarse = 32, kGroup = kDigits / kCoarse;
   extern __shared__ uint32_t s_order[];
   // Alone, counts of every pass; in a cluster two passes' in turn, so that four
   // CTAs fit an SM (48 KB each at 8192 slots): 89.1 us against 90.3.
@@ -211,15 +203,13 @@ __global__ void __launch_bounds__(kSelect)
 #pragma unroll 1
     for (int pass = 0; pass < kPasses; pass++) {
       if (need == 0) break;  // uniform in the cluster
-      const int shift = ONE ? 24 - 8 * pass : pass == 0 ? 21 : pass == 1 ? 10 : 0;
-      const int bits = ONE ? 8 : pass == 2 ? 10 : 11;
+      const int shift = D::shift(pass), bits = D::bits(pass);
       int* hist = s_hist[pass % kHists];
       if (pass > 0) {
 #pragma unroll 4
         for (int r = 0; r < rounds; r++) {
           const uint32_t o = order_at(r);
-          // The held ones (all bits set) share no prefix with a weight that competes.
-          if ((o ^ prefix) >> (shift + bits) == 0) atomicAdd(hist + (o >> shift & ((1 << bits) - 1)), 1);
+          if (counts(o, prefix, shift + bits)) atomicAdd(hist + (o >> shift & ((1 << bits) - 1)), 1);
         }
       }
       if (!ONE) {
@@ -330,7 +320,8 @@ __global__ void __launch_bounds__(kMoveThreads)
   if (count <= 0) return;
   if (threadIdx.x < count) {
     const int j = j0 + threadIdx.x;
-    const uint32_t old = a.kept[((size_t)i * a.key_heads + h) * a.keep + j];
+    // No word of `kept` leads outside the sequence, whoever wrote it.
+    const uint32_t old = min(a.kept[((size_t)i * a.key_heads + h) * a.keep + j], a.from.lens[i] - 1);
     const uint32_t from = (uint32_t)pool_row(a.from, i, (int)old, h, a.key_heads);
     const uint32_t to = (uint32_t)pool_row(a.to, i, j, h, a.key_heads);
     s_from[threadIdx.x] = from, s_to[threadIdx.x] = to;

@@ -677,3 +677,49 @@ def test_refusals(slm, ctx, ops):
     assert x.tolist() == [1.0] * 8
     attend()
     ctx.sync()
+
+
+def evicted(slm, ctx, ops, pool, keep, sinks, recent):
+    """An eviction of the whole pool's sequences, checked whole: kept slots, K, V, weights, lengths."""
+    lens, kh, page = pool.lens, pool.kh, pool.page
+    to_per = max(1, -(-min(max(lens), keep) // page))
+    to = slm.Table(ctx, len(lens), to_per, page, pool.pages)
+    to_ids = [pool.free[i * to_per:(i + 1) * to_per] for i in range(len(lens))]
+    for i, ids in enumerate(to_ids):
+        to.assign(i, ids)
+    kept = ops.zeros(len(lens) * kh * keep)
+    ops.paged_evict(kept, pool.kb, pool.vb, pool.wb, pool.table, to, keep=keep, sinks=sinks, recent=recent,
+                    key_heads=kh, dh=pool.dh, bf16=pool.bf16)
+    got = kept.read().view(np.uint32).reshape(len(lens), kh, keep)
+    k, v, w = pool.k.copy(), pool.v.copy(), pool.w.copy()
+    for i, n in enumerate(lens):
+        for h in range(kh):
+            ws = pool.rows(pool.w, i, 0, n)[h] if n else np.zeros(0, np.float32)
+            old = keep_slots(ws, n, keep, sinks, recent)
+            np.testing.assert_array_equal(got[i, h, :len(old)], old)
+            assert (got[i, h, len(old):] == 0xFFFFFFFF).all()
+            new = np.arange(len(old))
+            if len(old):
+                a = np.asarray(pool.ids[i])[old // page], h, old % page
+                b = np.asarray(to_ids[i])[new // page], h, new % page
+                k[b], v[b], w[b] = pool.k[a], pool.v[a], pool.w[a]
+    np.testing.assert_array_equal(pool.down(pool.kb), k)
+    np.testing.assert_array_equal(pool.down(pool.vb), v)
+    np.testing.assert_array_equal(pool.weights(), w)
+    np.testing.assert_array_equal(to.lens(), np.minimum(lens, keep))
+
+
+# A CTA a pair (short sequences; many pairs), and clusters.
+@pytest.mark.parametrize("lens,kh,keep,sinks,recent", [
+    ([300, 0, 17, 299], 2, 20, 2, 10), ([600, 1024, 513], 4, 512, 1, 64), ([300, 21], 1, 20, 0, 0),
+    ([(i * 97) % 1300 for i in range(100)], 3, 200, 4, 64), ([1500, 400, 3000], 2, 300, 4, 32), ([9000], 2, 500, 2, 100)])
+@pytest.mark.parametrize("large", [np.inf, np.finfo(np.float32).max, 2.0 ** 127])
+@pytest.mark.parametrize("share", [0.01, 0.2, 1.0])
+def test_evict_by_large_weights(slm, ctx, ops, lens, kh, keep, sinks, recent, large, share):
+    """Tokens pinned by +inf, and weights up to the largest: fewer, as many, more of them than places."""
+    rng = np.random.default_rng(50)
+    page = 16
+    pool = Pool(slm, ctx, ops, rng, lens, kh, 16, page, False, spare=len(lens) * -(-keep // page) + 1)
+    pool.w[rng.random(pool.w.shape) < share] = large
+    pool.wb = ops.upload(pool.w)
+    evicted(slm, ctx, ops, pool, keep, sinks, recent)
