@@ -238,7 +238,7 @@ int slm_op_paged_attend(slm_ctx* ctx, slm_buf* y, slm_buf* scores, const slm_buf
 /* Brings every sequence of `from` down to at most `keep` tokens per key head,
  * writing them to the pages of `to` (a table of the same sequences over the
  * same pool).  Per sequence and key head: up to `keep` tokens are all kept;
- * of more, the first `sinks`, the last `recent` (sinks + recent ≤ keep) and
+ * of more, the first `sinks`, the last `recent` (sinks + recent ≤ keep < 2^31) and
  * then those of the highest weight (equal weights: the lower slot first; NaN
  * below every number), in slot order.  K, V and weight rows are copied; the
  * rows they came from, and the rows of `to`'s pages behind the last kept

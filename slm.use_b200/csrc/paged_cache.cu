@@ -157,7 +157,8 @@ __global__ void __launch_bounds__(kSelect)
   const int n = (int)a.from.lens[i];
   uint32_t* out = a.kept + ((size_t)i * a.key_heads + h) * a.keep;
   if (n <= a.keep) {  // all kept; uniform in the cluster
-    for (int j = part * kSelect + t; j < a.keep; j += parts * kSelect) out[j] = j < n ? (uint32_t)j : 0xffffffffu;
+    const size_t keep = a.keep, step = parts * kSelect;  // a step past keep may pass 2^31
+    for (size_t j = part * kSelect + t; j < keep; j += step) out[j] = j < (size_t)n ? (uint32_t)j : 0xffffffffu;
   } else {
     for (int d = t; d < kHists * kDigits; d += kSelect) (&s_hist[0][0])[d] = 0;
     // A warp's slots lie together: 32 · rounds of them.

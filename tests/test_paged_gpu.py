@@ -723,3 +723,21 @@ def test_evict_by_large_weights(slm, ctx, ops, lens, kh, keep, sinks, recent, la
     pool.w[rng.random(pool.w.shape) < share] = large
     pool.wb = ops.upload(pool.w)
     evicted(slm, ctx, ops, pool, keep, sinks, recent)
+
+
+def test_evict_at_the_largest_budget(slm, ctx, ops):
+    """2^31 - 1 words of kept: the step after the last would pass 2^31."""
+    import torch
+    pool = Pool(slm, ctx, ops, np.random.default_rng(51), [5], 1, 8, 4, False)
+    to = slm.Table(ctx, 1, 2, 4, pool.pages)
+    to.assign(0, pool.free[:2])
+    kept, keep = ops.zeros(1), (1 << 31) - 1
+    ops.paged_evict(kept, pool.kb, pool.vb, pool.wb, pool.table, to, keep=keep, sinks=0, recent=0, key_heads=1, dh=8)
+    ctx.sync()
+
+    class Words:
+        __cuda_array_interface__ = {"shape": (keep,), "typestr": "<i4", "data": (kept.ptr, False), "version": 2}
+    got = torch.as_tensor(Words(), device="cuda")
+    assert got[:6].tolist() == [0, 1, 2, 3, 4, -1]
+    assert all(bool((part == -1).all()) for part in got[5:].split(1 << 28))
+    np.testing.assert_array_equal(to.lens(), [5])
