@@ -595,7 +595,8 @@ constexpr int kMaxTakers = 148 * kMaxCtas * kWarps;  // and pieces of a pair
 template <int kJoin>
 __device__ void join(const PagedAttendArgs& a, const Scratch& sc, const Work& wk, bool by_pair,
                      uint32_t x0, int y0) {
-  __shared__ float s_factor[kMaxTakers], s_red[2][kJoin / 32], s_sum[kJoin * 4];
+  __shared__ __align__(16) float s_sum[kJoin * 4];  // stored four at a time
+  __shared__ float s_factor[kMaxTakers], s_red[2][kJoin / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = a.heads / a.key_heads, per_key = (group + kHeads - 1) / kHeads;
   int seq, tile;
