@@ -180,7 +180,9 @@ int slm_op_attend_noalloc(slm_ctx* ctx, float* y, const float* q, const float* k
  * Every buffer and table must belong to the context of the call
  * (SLM_ERR_INVALID otherwise), no buffer may be passed twice, and a call
  * made while the context's stream is being captured fails with
- * SLM_ERR_INVALID.  Calls queue on the context's stream and read the table as
+ * SLM_ERR_INVALID (slm_table_new and slm_table_free too, which then makes and
+ * frees nothing; slm_table_assign, _set_lens and _lens touch the host's copy
+ * alone and may be called).  Calls queue on the context's stream and read the table as
  * it is when the call is made.                                             */
 /* ---------------------------------------------------------------------- */
 

@@ -317,8 +317,7 @@ class Table:
     def close(self):
         # The free function is looked up while the module is intact: at
         # interpreter exit its globals may already be gone.
-        if getattr(self, "_h", None):
-            self._free(self._h)
+        if getattr(self, "_h", None) and self._free(self._h) == 0:  # refused during a capture: still open
             self._h = None
 
     __del__ = close

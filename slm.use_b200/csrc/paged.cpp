@@ -105,6 +105,7 @@ int slm_table_new(slm_ctx* c, size_t seqs, size_t per_seq, size_t page, size_t p
   return guard([&] {
     SLM_REQUIRE(c && out, "table: bad arguments");
     Device dev(c);
+    not_capturing(c, "table_new");  // a captured clearing would empty the table at every replay
     auto* t = new slm_table{c, PageTable(seqs, per_seq, page, pages)};
     try {
       const size_t bytes = t->host.words.size() * sizeof(uint32_t);
@@ -127,6 +128,7 @@ int slm_table_free(slm_table* t) {
     slm_ctx* c = t->ctx;
     {
       Device dev(c);
+      not_capturing(c, "table_free");  // the wait below would end the capture
       cudaStreamSynchronize(c->stream);
       dev_free(t->dev);
     }

@@ -741,3 +741,43 @@ def test_evict_at_the_largest_budget(slm, ctx, ops):
     assert got[:6].tolist() == [0, 1, 2, 3, 4, -1]
     assert all(bool((part == -1).all()) for part in got[5:].split(1 << 28))
     np.testing.assert_array_equal(to.lens(), [5])
+
+
+@pytest.mark.parametrize("mode", ["relaxed", "thread_local"])
+def test_tables_are_neither_made_nor_freed_in_a_capture(slm, ctx, ops, mode):
+    """Both are refused, the capture stays usable, and the tables are as they were."""
+    import gc
+
+    import torch
+    rng = np.random.default_rng(52)
+    pool = Pool(slm, ctx, ops, rng, [20, 3], 2, 64, 16, False)
+    q = rng.standard_normal((2, 4, 64)).astype(np.float32)
+    qb = ops.upload(q)
+    stream, g = torch.cuda.ExternalStream(ctx.stream), torch.cuda.CUDAGraph()
+    x = torch.zeros(8, device="cuda")
+    x += 1
+    x.zero_()
+    ctx.sync()
+    torch.cuda.synchronize()
+    gc.collect()
+    gc.disable()  # a buffer freed during the capture would wait for the stream
+    try:
+        with torch.cuda.graph(g, stream=stream, capture_error_mode=mode):
+            x += 1
+            with pytest.raises(slm.SlmError, match="captured") as e:
+                slm.Table(ctx, 2, 4, 16, 64)
+            pool.table.close()
+            pool.table.set_lens([19, 4])
+    finally:
+        gc.enable()
+    assert e.value.code == 1
+    g.replay()
+    torch.cuda.synchronize()
+    assert x.tolist() == [1.0] * 8
+    pool.lens = [19, 4]
+    np.testing.assert_array_equal(pool.table.lens(), pool.lens)
+    y, tol, _ = pool.formula(q, 4, 0.125)
+    assert (abs(pool.attend(qb, 4, 0.125) - y) <= tol).all()
+    slm.Table(ctx, 2, 4, 16, 64).close()
+    pool.table.close()
+    assert pool.table._h is None
