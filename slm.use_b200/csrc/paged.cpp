@@ -21,29 +21,21 @@ struct slm_table {
 namespace slm {
 namespace {
 
-// Sends what changed since the last call, in stream order: few words in launch
-// parameters (a decode step's lengths and new pages; the host never waits),
-// many as one copy.
+// Sends what changed since the last call, in stream order.
 void flush(slm_table* t) {
   PageTable& h = t->host;
   if (h.changed.empty()) return;
-  constexpr size_t kFew = 4 * kPutWords;
-  std::vector<uint32_t> at, value;
-  for (const auto& c : h.changed)
-    for (size_t i = c.first; i < c.second && at.size() <= kFew; i++)
-      if (h.words[i] != t->sent[i]) at.push_back((uint32_t)i), value.push_back(h.words[i]);
+  const PageTable::Update u = h.update(t->sent);
   cudaStream_t st = t->ctx->stream;
-  if (at.size() <= kFew) {
-    for (size_t j = 0; j < at.size(); j += kPutWords)
-      table_put(t->dev, at.data() + j, value.data() + j, (int)std::min<size_t>(kPutWords, at.size() - j), st);
-    for (size_t j = 0; j < at.size(); j++) t->sent[at[j]] = value[j];
-  } else {
-    size_t lo = h.words.size(), hi = 0;
-    for (const auto& c : h.changed) lo = std::min(lo, c.first), hi = std::max(hi, c.second);
+  if (u.hi) {
     // Pageable source: the runtime has read it when the call returns.
-    SLM_CUDA(cudaMemcpyAsync(t->dev + lo, h.words.data() + lo, (hi - lo) * sizeof(uint32_t), cudaMemcpyHostToDevice,
-                             st));
-    std::copy(h.words.begin() + lo, h.words.begin() + hi, t->sent.begin() + lo);
+    SLM_CUDA(cudaMemcpyAsync(t->dev + u.lo, h.words.data() + u.lo, (u.hi - u.lo) * sizeof(uint32_t),
+                             cudaMemcpyHostToDevice, st));
+    std::copy(h.words.begin() + u.lo, h.words.begin() + u.hi, t->sent.begin() + u.lo);
+  } else {
+    for (size_t j = 0; j < u.at.size(); j += kPutWords)
+      table_put(t->dev, u.at.data() + j, u.value.data() + j, (int)std::min<size_t>(kPutWords, u.at.size() - j), st);
+    for (size_t j = 0; j < u.at.size(); j++) t->sent[u.at[j]] = u.value[j];
   }
   h.settle();
 }
