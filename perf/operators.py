@@ -108,7 +108,8 @@ _library = None
 
 
 def _slm():
-    """The library's Python mirror and one context's operators (the package folder has a dot in its name)."""
+    """The library's Python mirror and one context's operators (the package folder has a dot in its name).
+    torch works on the context's stream from then on, so what either queues is in order."""
     global _library
     if _library is None:
         import importlib.util
@@ -120,6 +121,8 @@ def _slm():
         sys.modules["slm_b200"] = slm
         spec.loader.exec_module(slm)
         ctx = slm.Context(0)
+        torch.cuda.synchronize()
+        torch.cuda.set_stream(torch.cuda.ExternalStream(ctx.stream))
         _library = slm, ctx, slm.Ops(ctx)
     return _library
 
@@ -167,17 +170,17 @@ def _inputs(case, seed):
 
 
 def prepare(case, seed):
+    if own:
+        slm, ctx, ops = _slm()
     state = dict(case=case, **_inputs(case, seed))
     if own:
         # What a user of the library holds: device buffers with the same contents, and the page tables.
-        slm, ctx, ops = _slm()
         n, page, per = case["n"], case["page"], state["table"].shape[1]
         pages = state["k"].shape[0]
         for name in ("k", "v", "q", "weights", "new_k", "new_v"):
             if name in state:
                 data = state[name]
                 buf = ops.zeros(-(-data.numel() * data.element_size() // 4))
-                ctx.sync()
                 state[name] = _seen(buf, data).copy_(data)
                 state[name + "_buf"] = buf
         state["ids"] = slm.Table(ctx, n, per, page, pages)
