@@ -219,7 +219,7 @@ typedef struct slm_paged {
  * would be negative (idle rows, a prompt shorter than m) are skipped.  The
  * table's lengths include the tokens stored.  bf16 pages hold the nearest
  * value, ties to even.  With `weights` (null: none) the stored tokens' weights
- * become 0.  Fails when a slot lies in a page that another sequence lists. */
+ * become 0, a prompt's too: only slm_op_paged_attend adds to them.  Fails when a slot lies in a page that another sequence lists. */
 int slm_op_paged_store(slm_ctx* ctx, slm_buf* k, slm_buf* v, slm_buf* weights, slm_table* table, size_t first,
                        size_t count, const slm_buf* ksrc, size_t koff, size_t ldk, const slm_buf* vsrc, size_t voff,
                        size_t ldv, size_t m, const slm_paged* p);
@@ -231,10 +231,14 @@ int slm_op_paged_store(slm_ctx* ctx, slm_buf* k, slm_buf* v, slm_buf* weights, s
  * least; a call that grows it waits for the calls before it).  With
  * `weights` (null: none) every visible token's weight grows by the sum of its
  * p over the query heads of its key head; fails when two sequences list one
- * page.  Arithmetic is f32 or better (page values as stored).  Slots outside
- * the visible range are not read; where a query, or a visible key or value,
- * is not finite or their products overflow f32, that sequence's results are
- * unspecified. */
+ * page.  Scores, softmax statistics and sums are f32.  Queries, probabilities
+ * and f32 keys and values enter products with 22 significant bits (bf16 ones
+ * as they are), and the exponential is good to 2^-22 and 0 below 2^-126: the
+ * results' errors are of the size of a plain f32 computation's.  Slots outside
+ * the visible range are not read.  A sequence's results are unspecified where
+ * a visible key or value, or a query times 1.45 · scale, is not finite, where
+ * the sizes of a score's products add up to more than f32 holds, or where a
+ * value passes 2^119 / visible tokens (sums are divided at the end). */
 int slm_op_paged_attend(slm_ctx* ctx, slm_buf* y, slm_buf* scores, const slm_buf* q, size_t qoff, size_t ldq,
                         const slm_buf* k, const slm_buf* v, slm_buf* weights, slm_table* table, const slm_paged* p);
 /* Brings every sequence of `from` down to at most `keep` tokens per key head,

@@ -4,8 +4,9 @@
 //
 // over the visible slots, in one pass: every warp keeps a running reference
 // maximum m, the sum l of exp(x - m) and the sum of exp(x - m) v, all f32.
-// Keys and values are read once, so bytes bound the call; the rest is arranged
-// to stay under them.
+// Keys and values are read once for every 8 query heads of a key head, so bytes
+// bound the call (but for many wide heads, see Shape); the rest is arranged to
+// stay under them.
 //
 // Work: the visible slots of every pair, a (sequence, tile of up to 8 query
 // heads of one key head), lie one after the other and are shared evenly over
@@ -14,19 +15,23 @@
 // so results do not depend on timing.  Where all pairs are short, a CTA's four
 // warps share one and join it themselves.
 //
-// Data: a warp streams its tiles through two or three private buffers with
+// Data: a warp streams its tiles through two to four private buffers with
 // 16-byte asynchronous copies, which look every row's page up (a page may end
 // anywhere in a tile) and fill rows past the end and columns past the head
-// size with zeros.  8 to 12 warps an SM keep about 100 KB in flight.
+// size with zeros.  8 to 12 warps an SM, 4 of 256-wide
+// f32 heads, keep 64 to 144 KB in flight.
 //
 // Products: mma.m16n8k8 on tf32, with the group's heads as rows.  Operands of
 // f32 precision are split into two tf32 parts, x = hi + lo: of the 16 rows, 8
 // hold the heads' hi parts and 8 their lo parts, so one product per part of
 // the other operand gives all four partial products, and a row pair's sum is
-// the f32 result.  bf16 keys and values are tf32 values as they are: one
-// product.  The tensor cores do in this form what the CUDA cores would do in
-// 8 times the instructions; a tcgen05 tile (64 or 128 rows) would be mostly
-// empty at 1 to 8 heads.
+// the result.  Two parts keep 22 of f32's 24 bits; three would leave room for 5
+// heads and take three products.  With two, errors against 64 bits are 2.0e-7
+// to 2.9e-7 on f32 pages, where plain f32 makes 2.0e-7 to 4.4e-7.  bf16 keys and
+// values are tf32 values as they are: one product.  The tensor cores do in this
+// form what the CUDA cores would do in 8 times the instructions.  With heads as
+// rows a tcgen05 tile (64 or 128 of them) would be mostly empty; slots as its
+// rows and heads times parts as columns would fill it, which is not built.
 #include <cuda_bf16.h>
 
 #include <algorithm>

@@ -781,3 +781,29 @@ def test_tables_are_neither_made_nor_freed_in_a_capture(slm, ctx, ops, mode):
     slm.Table(ctx, 2, 4, 16, 64).close()
     pool.table.close()
     assert pool.table._h is None
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("value,key", [(2.0 ** 106, 2.0 ** 60), (2.0 ** -60, 2.0 ** -60), (1.0, 2.0 ** 120)])
+def test_attend_with_large_and_small_values(slm, ctx, ops, bf16, value, key):
+    """Values up to 2^119 / visible tokens, and keys and queries whose sizes make up for one another."""
+    rng = np.random.default_rng(53)
+    pool = Pool(slm, ctx, ops, rng, [1000, 9], 2, 64, 16, bf16)
+    pool.k, pool.v = pool.k * np.float32(key), np.clip(pool.v, -4, 4) * np.float32(value)
+    pool.kb, pool.vb = pool.up(pool.k), pool.up(pool.v)
+    q = (rng.standard_normal((2, 6, 64)) / key).astype(np.float32)
+    y, tol, drawn = pool.formula(q, 6, 0.125)
+    got = pool.attend(ops.upload(q), 6, 0.125, weights=True)
+    assert (abs(got - y) <= tol).all(), float((abs(got - y) / tol).max())
+    pool.check_weights(pool.w, pool.weights(), drawn)
+
+
+def test_evicting_from_a_common_beginning(slm, ctx, ops):
+    """Two sequences that list the same first pages go to pages of their own; the shared ones stay."""
+    rng = np.random.default_rng(54)
+    pool = Pool(slm, ctx, ops, rng, [50, 40], 2, 64, 16, True, spare=8)
+    pool.table.set_lens([50, 0])
+    pool.ids[1] = pool.ids[0][:2] + pool.ids[1][2:]
+    pool.table.assign(1, pool.ids[1])
+    pool.table.set_lens(pool.lens)
+    evicted(slm, ctx, ops, pool, 24, 2, 8)
