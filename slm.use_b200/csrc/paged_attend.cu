@@ -898,7 +898,7 @@ void paged_attend(const PagedAttendArgs& a, cudaStream_t st) {
   if (!ctas) return;
   // Few pieces a pair: small CTAs, since there are many; 128 threads where the
   // weights of many query heads are added (12 a key head: 21.9 us against 26.1).
-  const bool few = p.work.takers < 32u * p.pairs && a.dh <= 128;
+  const bool few = p.work.takers / 32 < (uint32_t)p.pairs && a.dh <= 128;
   const int threads = !few ? 256 : a.weights && a.heads / a.key_heads > 4 ? 128 : 64;
   launch_after(threads == 64 ? k_paged_finish<64> : threads == 128 ? k_paged_finish<128> : k_paged_finish<256>,
                dim3(ctas), threads, 0, st, a, sc, p.work, by_pair, joins, heads, p.weight_slots);
