@@ -229,7 +229,8 @@ __global__ void __launch_bounds__(kSelect)
         // The digit, from the top, that holds the need-th largest: eight of them a lane.
         const int low = kDigits - 8 - 8 * lane;
         const int4 x = *reinterpret_cast<const int4*>(hist + low), y = *reinterpret_cast<const int4*>(hist + low + 4);
-        const int c[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        const int out_of = lane == 0 ? held_counted<ONE>(a.sinks + a.recent, prefix, pass) : 0;
+        const int c[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w - out_of};
         int all = 0;
 #pragma unroll
         for (int d = 0; d < 8; d++) all += c[d];
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(kSelect)
 #pragma unroll
           for (int d = 7; d > 0; d--)
             if (digit == low + d && c[d] < left) left -= c[d], digit--;
-          s_digit = digit, s_left = left, s_rest = hist[digit] - left;
+          s_digit = digit, s_left = left, s_rest = hist[digit] - (digit == low + 7 ? out_of : 0) - left;
         }
       } else if (warp == 0) {
         // The group of digits, then the digit, two of them a lane.

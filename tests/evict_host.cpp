@@ -19,6 +19,7 @@ int search(const float* w, int n, int keep, int sinks, int recent, uint32_t* out
     std::vector<int> hist(D::kCount, 0);
     for (uint32_t o : order)
       if (pass == 0 ? o != slm::kHeld : slm::counts(o, prefix, shift + bits)) hist[o >> shift & ((1 << bits) - 1)]++;
+    hist[(1 << bits) - 1] -= slm::held_counted<ONE>(sinks + recent, prefix, pass);
     int digit = D::kCount - 1;
     while (digit > 0 && hist[digit] < need) need -= hist[digit--];
     prefix |= (uint32_t)digit << shift;
