@@ -75,14 +75,14 @@ class PageTable {
   };
   Update update(const std::vector<uint32_t>& sent) const {
     Update u;
-    size_t lo = words.size(), hi = 0;
+    size_t lo = words.size(), hi = 0, marked = 0;
+    for (const auto& c : changed) lo = std::min(lo, c.first), hi = std::max(hi, c.second), marked += c.second - c.first;
+    const size_t most = hi - lo <= kUnheld ? kFew : kStep;
+    u.at.reserve(std::min(marked, most + 1)), u.value.reserve(std::min(marked, most + 1));
     for (const auto& c : changed)
-      for (size_t i = c.first; i < c.second; i++)
-        if (words[i] != sent[i]) {
-          lo = std::min(lo, i), hi = std::max(hi, i + 1);
-          if (u.at.size() <= kStep) u.at.push_back((uint32_t)i), u.value.push_back(words[i]);
-        }
-    if (u.at.size() > kFew && (hi - lo <= kUnheld || u.at.size() > kStep)) u.lo = lo, u.hi = hi;
+      for (size_t i = c.first; i < c.second && u.at.size() <= most; i++)
+        if (words[i] != sent[i]) u.at.push_back((uint32_t)i), u.value.push_back(words[i]);
+    if (u.at.size() > most) u.lo = lo, u.hi = hi;
     return u;
   }
 
