@@ -120,7 +120,10 @@ int slm_table_free(slm_table* t) {
     slm_ctx* c = t->ctx;
     {
       Device dev(c);
-      not_capturing(c, "table_free");  // the wait below would end the capture
+      // The wait below would end a capture.  A query that fails keeps no table from being freed.
+      cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+      cudaStreamIsCapturing(c->stream, &capture);
+      SLM_REQUIRE(capture == cudaStreamCaptureStatusNone, "table_free: the stream is being captured");
       cudaStreamSynchronize(c->stream);
       dev_free(t->dev);
     }
