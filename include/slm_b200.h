@@ -180,10 +180,10 @@ int slm_op_attend_noalloc(slm_ctx* ctx, float* y, const float* q, const float* k
  * Every buffer and table must belong to the context of the call
  * (SLM_ERR_INVALID otherwise), no buffer may be passed twice, and a call
  * made while the context's stream is being captured fails with
- * SLM_ERR_INVALID (slm_table_new and slm_table_free too, which then makes and
- * frees nothing; slm_table_assign, _set_lens and _lens touch the host's copy
- * alone and may be called).  Calls queue on the context's stream and read the table as
- * it is when the call is made.                                             */
+ * SLM_ERR_INVALID (slm_table_new and slm_table_free too, which then make and
+ * free nothing; slm_table_assign, _set_lens and _lens touch the host's copy
+ * alone and may be called).  Calls queue on the context's stream and read the
+ * table as it is when the call is made.                                    */
 /* ---------------------------------------------------------------------- */
 
 /* A table of `seqs` sequences of up to `per_seq` pages of `page` tokens, page
@@ -219,7 +219,8 @@ typedef struct slm_paged {
  * would be negative (idle rows, a prompt shorter than m) are skipped.  The
  * table's lengths include the tokens stored.  bf16 pages hold the nearest
  * value, ties to even.  With `weights` (null: none) the stored tokens' weights
- * become 0, a prompt's too: only slm_op_paged_attend adds to them.  Fails when a slot lies in a page that another sequence lists. */
+ * become 0, a prompt's too: only slm_op_paged_attend adds to them.  Fails when
+ * a slot lies in a page that another sequence lists. */
 int slm_op_paged_store(slm_ctx* ctx, slm_buf* k, slm_buf* v, slm_buf* weights, slm_table* table, size_t first,
                        size_t count, const slm_buf* ksrc, size_t koff, size_t ldk, const slm_buf* vsrc, size_t voff,
                        size_t ldv, size_t m, const slm_paged* p);
@@ -244,9 +245,9 @@ int slm_op_paged_attend(slm_ctx* ctx, slm_buf* y, slm_buf* scores, const slm_buf
 /* Brings every sequence of `from` down to at most `keep` tokens per key head,
  * writing them to the pages of `to` (a table of the same sequences over the
  * same pool).  Per sequence and key head: up to `keep` tokens are all kept;
- * of more, the first `sinks`, the last `recent` (sinks + recent ≤ keep < 2^31) and
- * then those of the highest weight (equal weights: the lower slot first; NaN
- * below every number), in slot order.  K, V and weight rows are copied; the
+ * of more, the first `sinks`, the last `recent` (sinks + recent ≤ keep < 2^31)
+ * and then those of the highest weight (equal weights: the lower slot first;
+ * NaN below every number), in slot order.  K, V and weight rows are copied; the
  * rows they came from, and the rows of `to`'s pages behind the last kept
  * token, stay as they were.  kept[i][key head][j] (32-bit words, seqs ×
  * key_heads × keep, grown as needed) is the slot in `from` that slot j of `to`

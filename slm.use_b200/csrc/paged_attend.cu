@@ -18,8 +18,8 @@
 // Data: a warp streams its tiles through two to four private buffers with
 // 16-byte asynchronous copies, which look every row's page up (a page may end
 // anywhere in a tile) and fill rows past the end and columns past the head
-// size with zeros.  8 to 12 warps an SM, 4 of 256-wide
-// f32 heads, keep 64 to 144 KB in flight.
+// size with zeros.  8 to 12 warps an SM (4 at 256-wide f32 heads) keep 64
+// to 144 KB in flight.
 //
 // Products: mma.m16n8k8 on tf32, with the group's heads as rows.  Operands of
 // f32 precision are split into two tf32 parts, x = hi + lo: of the 16 rows, 8
@@ -27,12 +27,12 @@
 // the other operand gives all four partial products, and a row pair's sum is
 // the result.  Two parts keep 22 of f32's 24 bits; three would leave room for 5
 // heads and take three products.  With two, errors against 64 bits are 1.5e-7
-// to 3.3e-7 on f32 pages, where plain f32 makes 0.6e-7 to 4.4e-7 (the smaller
-// the fewer tokens).  bf16 keys and
-// values are tf32 values as they are: one product.  The tensor cores do in this
-// form what the CUDA cores would do in 8 times the instructions.  With heads as
-// rows a tcgen05 tile (64 or 128 of them) would be mostly empty; slots as its
-// rows and heads times parts as columns would fill it, which is not built.
+// to 3.3e-7 on f32 pages, where plain f32 makes 0.6e-7 (a few tokens) to 4.4e-7
+// (16389).  bf16 keys and values are tf32 values as they are: one product.  The
+// tensor cores do in this form what the CUDA cores would do in 8 times the
+// instructions.  With heads as rows a tcgen05 tile (64 or 128 of them) would be
+// mostly empty; slots as its rows and heads times parts as columns would fill
+// it, which is not built.
 #include <cuda_bf16.h>
 
 #include <algorithm>
