@@ -26,9 +26,10 @@
 // hold the heads' hi parts and 8 their lo parts, so one product per part of
 // the other operand gives all four partial products, and a row pair's sum is
 // the result.  Two parts keep 22 of f32's 24 bits; three would leave room for 5
-// heads and take three products.  With two, errors against 64 bits are 1.5e-7
-// to 3.3e-7 on f32 pages, where plain f32 makes 0.6e-7 (a few tokens) to 4.4e-7
-// (16389).  bf16 keys and values are tf32 values as they are: one product.  The
+// heads and take three products.  Errors against 64 bits on f32 pages (in
+// brackets those of plain f32, 64-wide heads): 0.8e-7 of one token (0), 2.0e-7
+// of 8 (1.6e-7), 2.8e-7 of 97 (2.9e-7), 2.9e-7 of 16389 (4.3e-7).  bf16 keys and
+// values are tf32 values as they are: one product, errors of 0 to 2.0e-7.  The
 // tensor cores do in this form what the CUDA cores would do in 8 times the
 // instructions.  With heads as rows a tcgen05 tile (64 or 128 of them) would be
 // mostly empty; slots as its rows and heads times parts as columns would fill
