@@ -188,7 +188,8 @@ int slm_op_attend_noalloc(slm_ctx* ctx, float* y, const float* q, const float* k
 
 /* A table of `seqs` sequences of up to `per_seq` pages of `page` tokens, page
  * ids below `pages`.  Every sequence starts without pages, at length 0.
- * Limits: seqs ≤ 4096, per_seq · page < 2^30, pages < 2^31. */
+ * Limits: seqs ≤ 4096, per_seq · page < 2^30, pages < 2^31, seqs · (per_seq +
+ * 1) < 2^32. */
 int slm_table_new(slm_ctx* ctx, size_t seqs, size_t per_seq, size_t page, size_t pages, slm_table** out);
 int slm_table_free(slm_table* table);
 /* Sequence `seq` has the n pages ids[0..n): slot s is row s % page of page
